@@ -1,0 +1,376 @@
+"""The operators that a decoder or long-document backbone needs next to the encoder's own, as cases that can be run and timed:
+
+* attention over packed sequences with grouped heads, causal or within a window (``ops.attn_gqa_fwd`` / ``ops.attn_gqa_bwd``);
+* the scaled embedding lookup and its gradient by sorted tokens (``ops.embed_fwd`` / ``ops.embed_bwd``);
+* dropout with a counter-based mask that is never stored (``ops.dropout_fwd`` / ``ops.dropout_bwd``).
+
+``run`` computes them in their plain form (elementary torch operations in fp32, rounded once at the end) or, where ``own`` is true,
+through this package.  ``exact`` is the definition in 64 bits."""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+BYTES = {"bf16": 2, "fp16": 2, "fp32": 4}
+
+
+# ------------------------------------------------------------------------------------------------ cases
+def _attn(name, op, B, lo, hi, heads, kv_heads, dim, dtype="bf16", causal=False, left=-1, right=-1, mask=False, tail=0, lseed=1):
+    """B packed sequences of lo .. hi tokens (log-uniform, fixed by lseed), `tail` rows of the buffer behind the last of them"""
+    c = {"op": op, "B": B, "lo": lo, "hi": hi, "heads": heads, "kv_heads": kv_heads, "dim": dim, "dtype": dtype, "causal": causal,
+         "left": left, "right": right, "mask": mask, "tail": tail, "lseed": lseed}
+    return dict(c, name=name) if name else c
+
+
+def listed():
+    return [
+        # a few search queries on their way through a 12-head encoder: latency
+        _attn("attn fwd queries", "attn_fwd", 8, 1, 32, 12, 12, 64),
+        # a corpus-encoding batch of ragged passages, 16 heads, some keys masked out
+        _attn("attn fwd passages", "attn_fwd", 256, 20, 256, 16, 16, 64, mask=True, lseed=2),
+        # one long document through a decoder with grouped heads
+        _attn("attn fwd document", "attn_fwd", 1, 8192, 8192, 32, 8, 128, causal=True),
+        # the contrastive training step's batch: 64 sequences of 128 tokens, 12 heads
+        _attn("attn train spans", "attn_train", 64, 128, 128, 12, 12, 64),
+        # decoder training on ragged packed text, one token to 2048, grouped heads
+        _attn("attn train ragged", "attn_train", 16, 1, 2048, 32, 8, 128, causal=True, lseed=3),
+        # long documents in an encoder with local attention, fp16, masked keys, odd lengths
+        _attn("attn train local", "attn_train", 3, 2047, 4099, 12, 12, 64, dtype="fp16", left=64, right=64, mask=True, lseed=4),
+        # decoder training on long sequences: the largest
+        _attn("attn train long", "attn_train", 4, 4096, 4096, 32, 8, 128, causal=True),
+        # the lookup of the 64 x 128 training batch from the fp32 master table
+        {"name": "embed fwd batch", "op": "embed_fwd", "n": 8192, "vocab": 30522, "width": 768, "table": "fp32", "dtype": "bf16", "pad": 0.0},
+        # its gradient: natural text, where a few tokens make up most of the rows
+        {"name": "embed bwd batch", "op": "embed_bwd", "n": 8192, "vocab": 30522, "width": 768, "table": "fp32", "dtype": "bf16", "pad": 0.0},
+        # the gradient of a large vocabulary's table, with padding rows
+        {"name": "embed bwd large", "op": "embed_bwd", "n": 32768, "vocab": 65536, "width": 2048, "table": "fp32", "dtype": "bf16", "pad": 0.1},
+        # the residual dropout of a handful of queries: latency
+        {"name": "dropout fwd queries", "op": "dropout_fwd", "rows": 256, "width": 768, "dtype": "bf16", "residual": True, "p": 0.1},
+        # the gradient through the residual dropout of a long batch
+        {"name": "dropout bwd long", "op": "dropout_bwd", "rows": 16384, "width": 4096, "dtype": "bf16", "residual": False, "p": 0.1},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["attn_fwd", "attn_train", "attn_train", "embed_fwd", "embed_bwd", "dropout_fwd", "dropout_bwd"])
+    if op.startswith("attn"):
+        dim = rng.choice([32, 64, 64, 80, 96, 128, 128])
+        kv = rng.choice([1, 2, 4, 8, 12])
+        group = rng.choice([1, 1, 2, 4])
+        hi = _log_int(rng, 1, 4096)
+        lo = max(1, int(hi * rng.choice([0.02, 0.3, 1.0])))
+        # scores (half of heads * B * hi^2 there: it is causal) and traffic (the tokens' queries and keys) stay below the largest listed case's
+        heads = kv * group
+        most = max(1, min(256, int(32 * 4 * 4096 * 4096 / (2 * heads * hi * hi)), int(16384 * (5 * 32 + 6 * 8) * 128 / (hi * (5 * heads + 6 * kv) * dim))))
+        B = _log_int(rng, 1, most)
+        causal = rng.random() < 0.5
+        left = rng.choice([-1, -1, 0, 16, 128, 1000])
+        right = 0 if causal else rng.choice([-1, -1, 0, 16, 128, 1000]) if left >= 0 else -1
+        return _attn(None, op, B, lo, hi, heads, kv, dim, rng.choice(["bf16", "bf16", "fp16"]), causal, left, -1 if causal else right,
+                     rng.random() < 0.3, rng.choice([0, 0, 5, 37]), rng.randrange(1 << 20))
+    if op.startswith("embed"):
+        width = 8 * _log_int(rng, 4, 512)
+        return {"op": op, "n": _log_int(rng, 1, 32768), "vocab": _log_int(rng, 16, min(131072, 65536 * 1792 // width)), "width": width,
+                "table": rng.choice(["fp32", "fp32", "bf16", "fp16"]), "dtype": rng.choice(["bf16", "fp16", "fp32"]),
+                "pad": rng.choice([0.0, 0.0, 0.2])}
+    return {"op": op, "rows": _log_int(rng, 1, 16384), "width": _log_int(rng, 1, 4096), "dtype": rng.choice(["bf16", "bf16", "fp16", "fp32"]),
+            "residual": op == "dropout_fwd" and rng.random() < 0.6, "p": rng.choice([0.05, 0.1, 0.3])}
+
+
+def _lens(case):
+    r = random.Random(case["lseed"])
+    lens = [_log_int(r, case["lo"], case["hi"]) for _ in range(case["B"])]
+    lens[r.randrange(case["B"])] = case["hi"]
+    return lens
+
+
+def _window(case):
+    return case["left"], (0 if case["causal"] else case["right"])
+
+
+def _pairs(case):
+    """visible (query, key) pairs of one head, before the key mask"""
+    left, right = _window(case)
+    total = 0
+    for n in _lens(case):
+        i = np.arange(n, dtype=np.int64)
+        a = np.zeros_like(i) if left < 0 else np.maximum(i - left, 0)
+        b = np.full_like(i, n) if right < 0 else np.minimum(i + right + 1, n)
+        total += int((b - a).sum())
+    return total
+
+
+def work(case):
+    op = case["op"]
+    if op.startswith("attn"):
+        T, Hq, Hk, D, e = sum(_lens(case)), case["heads"], case["kv_heads"], case["dim"], BYTES[case["dtype"]]
+        q, kv, stat, small = T * Hq * D * e, 2 * T * Hk * D * e, 4 * T * Hq, 4 * (case["B"] + 1) + (4 * T if case["mask"] else 0)
+        fwd, products = q + kv + q + stat + small, 4
+        if op == "attn_fwd":
+            return {"bytes": fwd, "flops": products * D * Hq * _pairs(case)}
+        # the backward: the scores again and dP, dV, dQ, dK
+        return {"bytes": fwd + (q + kv + 2 * q + stat + small) + (q + kv), "flops": (products + 10) * D * Hq * _pairs(case)}
+    if op == "embed_fwd":
+        n, w = case["n"], case["width"]
+        return {"bytes": n * (4 + w * (BYTES[case["table"]] + BYTES[case["dtype"]])), "flops": n * w}
+    if op == "embed_bwd":
+        n, w = case["n"], case["width"]
+        return {"bytes": n * (4 + w * BYTES[case["dtype"]]) + case["vocab"] * w * 4, "flops": n * w}
+    n = case["rows"] * case["width"]
+    return {"bytes": n * BYTES[case["dtype"]] * (3 if case["residual"] else 2), "flops": n * (3 if case["residual"] else 2)}
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _normal(shape, dtype, g, scale=1.0):
+    return (torch.randn(shape, generator=g, device="cuda", dtype=torch.float32) * scale).to(dtype)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    op, dt = case["op"], DTYPES[case["dtype"]]
+    st = {"case": case}
+    if op.startswith("attn"):
+        lens = _lens(case)
+        Hq, Hk, D = case["heads"], case["kv_heads"], case["dim"]
+        T = sum(lens) + case["tail"]
+        # what a fused projection leaves: Q | K | V side by side in one row per token
+        st["qkv"] = _normal((T, (Hq + 2 * Hk) * D), dt, g)
+        st["q"], st["k"], st["v"] = (x.unflatten(1, (-1, D)) for x in st["qkv"].split((Hq * D, Hk * D, Hk * D), 1))
+        st["seq_off"] = torch.tensor(np.concatenate([[0], np.cumsum(lens)]), dtype=torch.int32, device="cuda")
+        st["lens"], st["longest"] = lens, max(lens)
+        st["mask"] = None
+        if case["mask"]:  # a tenth of the keys, and every key of one sequence where there are several
+            st["mask"] = (torch.rand(T, generator=g, device="cuda") >= 0.1).to(torch.int32)
+            if len(lens) > 1:
+                b = seed % len(lens)
+                st["mask"][sum(lens[:b]):sum(lens[:b + 1])] = 0
+        if op == "attn_train":
+            st["dctx"] = _normal((T, Hq, D), dt, g)
+        return st
+    if op.startswith("embed"):
+        n, V, w = case["n"], case["vocab"], case["width"]
+        u = torch.rand(n, generator=g, device="cuda", dtype=torch.float64)
+        ids = (torch.exp(u * math.log(V + 1)) - 1).floor().clamp_(0, V - 1)  # density ~ 1 / rank, as the words of a text
+        ids = torch.randperm(V, generator=g, device="cuda")[ids.long()]
+        if case["pad"]:
+            ids = torch.where(torch.rand(n, generator=g, device="cuda") < case["pad"], -1, ids)
+        st["ids"] = ids.to(torch.int32)
+        st["scale"] = math.sqrt(w)
+        if op == "embed_fwd":
+            st["table"] = _normal((V, w), DTYPES[case["table"]], g, 0.02)
+        else:
+            st["dout"] = _normal((n, w), dt, g)
+        return st
+    st["x"] = _normal((case["rows"], case["width"]), dt, g)
+    st["residual"] = _normal((case["rows"], case["width"]), dt, g) if case["residual"] else None
+    st["key"] = (seed * 7919 + 13, seed % 1000, seed % 24)  # the model's seed, the number of the step, the layer
+    return st
+
+
+# ------------------------------------------------------------------------------------------------ one pass
+def run(state):
+    case = state["case"]
+    return (_run_own if own else _run_plain)(state, case, case["op"])
+
+
+def _run_own(state, case, op):
+    from cocodr_amd import ops
+    if op.startswith("attn"):
+        q, k, v, off = state["q"], state["k"], state["v"], state["seq_off"]
+        how = dict(causal=case["causal"], window=(case["left"], case["right"]), mask=state["mask"])
+        ctx, lse = ops.attn_gqa_fwd(q, k, v, off, **how)
+        if op == "attn_fwd":
+            return {"ctx": ctx, "lse": lse}
+        dq, dk, dv = ops.attn_gqa_bwd(q, k, v, ctx, state["dctx"], lse, off, **how)
+        return {"ctx": ctx, "lse": lse, "dq": dq, "dk": dk, "dv": dv}
+    if op == "embed_fwd":
+        return ops.embed_fwd(state["ids"], state["table"], scale=state["scale"], out_dtype=DTYPES[case["dtype"]])
+    if op == "embed_bwd":
+        return ops.embed_bwd(state["dout"], state["ids"], case["vocab"], scale=state["scale"])
+    seed, call, layer = state["key"]
+    drop = ops.dropout_mask(case["p"], seed, call, layer, ops.KIND_FFN_OUT)
+    if op == "dropout_fwd":
+        return ops.dropout_fwd(state["x"], drop, residual=state["residual"])
+    return ops.dropout_bwd(state["x"], drop)
+
+
+def _run_plain(state, case, op):
+    if op.startswith("attn"):
+        return _plain_attention(state, case, op)
+    if op == "embed_fwd":
+        ids = state["ids"].long()
+        rows = state["table"][ids.clamp(min=0)].float() * state["scale"]
+        return torch.where(ids.unsqueeze(1) >= 0, rows, 0.0).to(DTYPES[case["dtype"]])
+    if op == "embed_bwd":
+        V = case["vocab"]
+        ids = state["ids"].long()
+        grad = torch.zeros((V + 1, case["width"]), dtype=torch.float32, device="cuda")
+        grad.index_add_(0, torch.where(ids < 0, V, ids), state["dout"].float() * state["scale"])
+        return grad[:V]
+    return _plain_dropout(state, case)
+
+
+def _plain_attention(state, case, op):
+    q, k, v, off = state["q"], state["k"], state["v"], state["seq_off"].long()
+    T, Hq, D = q.shape
+    Hk, L = case["kv_heads"], state["longest"]
+    G = Hq // Hk
+    scale = 1.0 / math.sqrt(D)
+    # padded copies [B, heads, L, D] of the packed rows, the keys and values once per query head
+    pos = torch.arange(L, device="cuda")
+    rows = off[:-1, None] + pos
+    real = rows < off[1:, None]
+    rows = rows.clamp(max=T - 1)
+    q32 = q[rows].float().transpose(1, 2).contiguous()
+    k32 = k[rows].float().transpose(1, 2).repeat_interleave(G, 1)
+    v32 = v[rows].float().transpose(1, 2).repeat_interleave(G, 1)
+    seen = real[:, None, :] & real[:, :, None]
+    left, right = _window(case)
+    if left >= 0:
+        seen = seen & (pos[None, :] >= pos[:, None] - left)
+    if right >= 0:
+        seen = seen & (pos[None, :] <= pos[:, None] + right)
+    if state["mask"] is not None:
+        seen = seen & (state["mask"][rows] != 0)[:, None, :]
+    seen = seen[:, None]
+    s = torch.matmul(q32, k32.transpose(2, 3).contiguous()).mul_(scale).masked_fill_(~seen, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = s.sub_(torch.where(top == -math.inf, 0.0, top)).exp_()
+    total = p.sum(-1, keepdim=True)
+    lse = (top + total.log()).squeeze(-1)
+    p.div_(torch.where(total == 0, 1.0, total))
+    o = torch.matmul(p, v32)
+    to = torch.where(real, rows, T).reshape(-1)  # rows of no sequence land behind the buffer
+
+    def packed(x, dtype, fill=0.0):
+        out = torch.full((T + 1,) + tuple(x.shape[2:]), fill, dtype=x.dtype, device="cuda")
+        out[to] = x.reshape((-1,) + tuple(x.shape[2:]))
+        return out[:T].to(dtype)
+
+    dt = q.dtype
+    out = {"ctx": packed(o.transpose(1, 2), dt), "lse": packed(lse.transpose(1, 2), torch.float32, -math.inf).t().contiguous()}
+    if op == "attn_fwd":
+        return out
+    do = torch.where(real[:, :, None, None], state["dctx"][rows].float(), 0.0).transpose(1, 2).contiguous()
+    dv = torch.matmul(p.transpose(2, 3), do)
+    ds = torch.matmul(do, v32.transpose(2, 3).contiguous()).sub_((do * o).sum(-1, keepdim=True)).mul_(p).mul_(scale)
+    dq = torch.matmul(ds, k32)
+    dk = torch.matmul(ds.transpose(2, 3), q32)
+    out["dq"] = packed(dq.transpose(1, 2), dt)
+    out["dk"] = packed(dk.unflatten(1, (Hk, G)).sum(2).transpose(1, 2), dt)
+    out["dv"] = packed(dv.unflatten(1, (Hk, G)).sum(2).transpose(1, 2), dt)
+    return out
+
+
+def _mix64(x):
+    m = (1 << 64) - 1
+    x = (x + 0x9E3779B97F4A7C15) & m
+    x = ((x ^ x >> 30) * 0xBF58476D1CE4E5B9) & m
+    x = ((x ^ x >> 27) * 0x94D049BB133111EB) & m
+    return x ^ x >> 31
+
+
+def _drop_numbers(case, key):
+    """(k0, k1, threshold, scale): the two keys of the mask, the 16-bit value below which an element is dropped, what the others are multiplied by"""
+    seed, call, layer = key
+    z = _mix64((seed + 0x9E3779B97F4A7C15 * (call + 1)) & ((1 << 64) - 1))
+    z = _mix64(z ^ ((0xD1B54A32D192ED03 * (4 * layer + 2 + 1)) & ((1 << 64) - 1)))  # site 2 of the layer: the output of its feed-forward part
+    threshold = int(math.floor(case["p"] * 65536 + 0.5))
+    return z & 0xFFFFFFFF, z >> 32, threshold, 65536.0 / (65536 - threshold)
+
+
+def _plain_dropout(state, case):
+    x = state["x"]
+    k0, k1, threshold, scale = _drop_numbers(case, state["key"])
+    i = torch.arange(x.numel(), dtype=torch.int64, device="cuda")
+    w = (i >> 1) ^ k0
+    w = w ^ (w >> 16)
+    w = (w * 0x7FEB352D) & 0xFFFFFFFF
+    w = w ^ (w >> 15)
+    w = (w * 0x846CA68B) & 0xFFFFFFFF
+    w = (w ^ (w >> 16)) ^ k1
+    u = torch.where((i & 1) != 0, w >> 16, w & 0xFFFF)
+    y = torch.where((u >= threshold).view(x.shape), x.float() * scale, 0.0)
+    if state["residual"] is not None:
+        y = y + state["residual"].float()
+    return y.to(x.dtype)
+
+
+# ------------------------------------------------------------------------------------------------ 64 bits
+def exact(case, seed):
+    st = prepare(case, seed)
+    op = case["op"]
+    if op.startswith("attn"):
+        return _exact_attention(st, case, op)
+    if op == "embed_fwd":
+        ids = st["ids"].cpu().numpy()
+        out = st["table"].double()[torch.from_numpy(np.maximum(ids, 0)).long().cuda()] * st["scale"]
+        out[torch.from_numpy(ids < 0).cuda()] = 0.0
+        return out
+    if op == "embed_bwd":
+        out = torch.zeros((case["vocab"], case["width"]), dtype=torch.float64, device="cuda")
+        ok = st["ids"] >= 0
+        return out.index_put_((st["ids"][ok].long(),), st["dout"][ok].double() * st["scale"], accumulate=True)
+    x = st["x"].double().cpu().numpy()
+    k0, k1, threshold, scale = _drop_numbers(case, st["key"])
+    w = np.arange((x.size + 1) // 2, dtype=np.uint32) ^ np.uint32(k0)
+    w ^= w >> np.uint32(16)
+    w *= np.uint32(0x7FEB352D)
+    w ^= w >> np.uint32(15)
+    w *= np.uint32(0x846CA68B)
+    w ^= w >> np.uint32(16)
+    w ^= np.uint32(k1)
+    keep = (np.stack([w & np.uint32(0xFFFF), w >> np.uint32(16)], 1).reshape(-1)[:x.size] >= threshold).reshape(x.shape)
+    y = x * np.where(keep, scale, 0.0)
+    return y + st["residual"].double().cpu().numpy() if st["residual"] is not None else y
+
+
+def _exact_attention(st, case, op):
+    """one sequence and one group of heads at a time; the gradients by differentiating the definition"""
+    T, Hq, D = st["q"].shape
+    Hk = case["kv_heads"]
+    G = Hq // Hk
+    left, right = _window(case)
+    f64 = dict(dtype=torch.float64, device="cuda")
+    out = {"ctx": torch.zeros((T, Hq, D), **f64), "lse": torch.full((Hq, T), -math.inf, **f64)}
+    if op == "attn_train":
+        out.update(dq=torch.zeros((T, Hq, D), **f64), dk=torch.zeros((T, Hk, D), **f64), dv=torch.zeros((T, Hk, D), **f64))
+    a = 0
+    for n in st["lens"]:
+        e = a + n
+        i = torch.arange(n, device="cuda")
+        gap = i[None, :] - i[:, None]  # how far the key lies behind the query
+        hidden = torch.zeros((n, n), dtype=torch.bool, device="cuda")
+        if left >= 0:
+            hidden |= gap < -left
+        if right >= 0:
+            hidden |= gap > right
+        if st["mask"] is not None:
+            hidden |= (st["mask"][a:e] == 0)[None, :]
+        void = hidden.all(1)
+        step = Hk if Hq * n * n <= 1 << 25 else 1
+        for h in range(0, Hk, step):
+            hq = slice(h * G, (h + step) * G)
+            q, k, v = (x.double().detach().requires_grad_(op == "attn_train") for x in (st["q"][a:e, hq], st["k"][a:e, h:h + step], st["v"][a:e, h:h + step]))
+            qh = q.reshape(n, step, G, D).permute(1, 2, 0, 3).reshape(step, G * n, D)
+            s = (torch.bmm(qh, k.permute(1, 2, 0).contiguous()) / math.sqrt(D)).view(step, G, n, n)
+            s = s.masked_fill(hidden, -math.inf)
+            out["lse"][hq, a:e] = torch.logsumexp(s.detach(), -1).reshape(step * G, n)
+            s = s.masked_fill(void[:, None], 0.0)
+            p = torch.softmax(s, -1) * (~void)[:, None]
+            o = torch.bmm(p.view(step, G * n, n), v.permute(1, 0, 2).contiguous()).view(step, G, n, D).permute(2, 0, 1, 3).reshape(n, step * G, D)
+            out["ctx"][a:e, hq] = o.detach()
+            if op == "attn_train":
+                dq, dk, dv = torch.autograd.grad(o, (q, k, v), st["dctx"][a:e, hq].double())
+                out["dq"][a:e, hq], out["dk"][a:e, h:h + step], out["dv"][a:e, h:h + step] = dq, dk, dv
+        a = e
+    return out
