@@ -14,14 +14,14 @@ import torch
 
 own = False
 
-DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
-BYTES = {"bf16": 2, "fp16": 2, "fp32": 4}
+DTYPES = {"bf16": torch.bfloat16, "fp32": torch.float32}  # what the package trains in: bf16 activations, fp32 masters
+BYTES = {"bf16": 2, "fp32": 4}
 
 
 # ------------------------------------------------------------------------------------------------ cases
-def _attn(name, op, B, lo, hi, heads, kv_heads, dim, dtype="bf16", causal=False, left=-1, right=-1, mask=False, tail=0, lseed=1):
+def _attn(name, op, B, lo, hi, heads, kv_heads, dim, causal=False, left=-1, right=-1, mask=False, tail=0, lseed=1):
     """B packed sequences of lo .. hi tokens (log-uniform, fixed by lseed), `tail` rows of the buffer behind the last of them"""
-    c = {"op": op, "B": B, "lo": lo, "hi": hi, "heads": heads, "kv_heads": kv_heads, "dim": dim, "dtype": dtype, "causal": causal,
+    c = {"op": op, "B": B, "lo": lo, "hi": hi, "heads": heads, "kv_heads": kv_heads, "dim": dim, "dtype": "bf16", "causal": causal,
          "left": left, "right": right, "mask": mask, "tail": tail, "lseed": lseed}
     return dict(c, name=name) if name else c
 
@@ -38,8 +38,8 @@ def listed():
         _attn("attn train spans", "attn_train", 64, 128, 128, 12, 12, 64),
         # decoder training on ragged packed text, one token to 2048, grouped heads
         _attn("attn train ragged", "attn_train", 16, 1, 2048, 32, 8, 128, causal=True, lseed=3),
-        # long documents in an encoder with local attention, fp16, masked keys, odd lengths
-        _attn("attn train local", "attn_train", 3, 2047, 4099, 12, 12, 64, dtype="fp16", left=64, right=64, mask=True, lseed=4),
+        # long documents in an encoder with local attention, masked keys, odd lengths
+        _attn("attn train local", "attn_train", 3, 2047, 4099, 12, 12, 64, left=64, right=64, mask=True, lseed=4),
         # decoder training on long sequences: the largest
         _attn("attn train long", "attn_train", 4, 4096, 4096, 32, 8, 128, causal=True),
         # the lookup of the 64 x 128 training batch from the fp32 master table
@@ -74,14 +74,14 @@ def draw(rng):
         causal = rng.random() < 0.5
         left = rng.choice([-1, -1, 0, 16, 128, 1000])
         right = 0 if causal else rng.choice([-1, -1, 0, 16, 128, 1000]) if left >= 0 else -1
-        return _attn(None, op, B, lo, hi, heads, kv, dim, rng.choice(["bf16", "bf16", "fp16"]), causal, left, -1 if causal else right,
+        return _attn(None, op, B, lo, hi, heads, kv, dim, causal, left, -1 if causal else right,
                      rng.random() < 0.3, rng.choice([0, 0, 5, 37]), rng.randrange(1 << 20))
     if op.startswith("embed"):
         width = 8 * _log_int(rng, 4, 512)
         return {"op": op, "n": _log_int(rng, 1, 32768), "vocab": _log_int(rng, 16, min(131072, 65536 * 1792 // width)), "width": width,
-                "table": rng.choice(["fp32", "fp32", "bf16", "fp16"]), "dtype": rng.choice(["bf16", "fp16", "fp32"]),
+                "table": rng.choice(["fp32", "fp32", "bf16"]), "dtype": rng.choice(["bf16", "bf16", "fp32"]),
                 "pad": rng.choice([0.0, 0.0, 0.2])}
-    return {"op": op, "rows": _log_int(rng, 1, 16384), "width": _log_int(rng, 1, 4096), "dtype": rng.choice(["bf16", "bf16", "fp16", "fp32"]),
+    return {"op": op, "rows": _log_int(rng, 1, 16384), "width": _log_int(rng, 1, 4096), "dtype": rng.choice(["bf16", "bf16", "fp32"]),
             "residual": op == "dropout_fwd" and rng.random() < 0.6, "p": rng.choice([0.05, 0.1, 0.3])}
 
 
