@@ -80,6 +80,13 @@ class EncoderBwdLayout(C.Structure):  # mirrors cocodr_encoder_bwd_layout_t
     _fields_ = [(n, c_size_t) for n in ("dy2", "du", "dy1", "dqkv", "ln2_partial", "ln1_partial")] + [("ln_blocks", c_int), ("ln_rows", c_int)]
 
 
+class AttnGqaArgs(C.Structure):  # mirrors cocodr_attn_gqa_args
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "seq_off", "mask")]
+                + [(n, c_longlong) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head", "do_row", "do_head",
+                                             "dq_row", "dq_head", "dk_row", "dk_head", "dv_row", "dv_head")]
+                + [(n, c_int) for n in ("T", "B", "heads", "kv_heads", "dim", "left", "right")] + [("scale", c_float)])
+
+
 EPI_NONE, EPI_GELU, EPI_ADD, EPI_DGELU = 0, 1, 2, 3
 
 # name -> (restype, argtypes); every symbol include/cocodr.h declares
@@ -116,6 +123,9 @@ SIGNATURES = {
     "cocodr_encoder_bwd_packed": (c_int, [C.POINTER(Config), C.POINTER(EmbedParams), C.POINTER(LayerParams), C.POINTER(EmbedGrads),
                                           C.POINTER(LayerGrads), C.POINTER(PackedBatch), c_void_p, c_void_p, c_size_t, c_int, c_int, c_int,
                                           c_void_p]),
+    "cocodr_attn_gqa_fwd": (c_int, [C.POINTER(AttnGqaArgs), c_void_p, c_void_p, c_int, c_void_p]),
+    "cocodr_attn_gqa_bwd_workspace_floats": (c_size_t, [C.POINTER(AttnGqaArgs)]),
+    "cocodr_attn_gqa_bwd": (c_int, [C.POINTER(AttnGqaArgs)] + [c_void_p] * 6 + [c_int, c_void_p, c_size_t, c_void_p]),
     "cocodr_embed_ln_fwd": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int, c_int, c_float, c_void_p]),
     "cocodr_embed_bwd_partial_floats": (c_size_t, [c_int, c_int]),
     "cocodr_embed_ln_bwd": (c_int, [c_void_p] * 14 + [c_int, c_int, c_int, c_int, c_void_p]),

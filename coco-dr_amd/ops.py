@@ -173,6 +173,101 @@ def attn_bwd(qkv, mask, ctx, dctx, lse, B: int, L: int, heads: int, qk_bias: boo
     return (dqkv, part) if qk_bias else dqkv
 
 
+# ----------------------------------------------------------------------------------------------- attention with grouped heads
+def _rows3(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
+    """a bf16 [T, heads, dim] tensor or view whose last dimension is contiguous"""
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: expected a tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: must live on the GPU (got {t.device}); this path has no CPU fallback")
+    if t.dtype != BF16:
+        raise ValueError(f"{name}: expected dtype {BF16}, got {t.dtype}")
+    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
+        raise ValueError(f"{name}: expected shape {shape or '[T, heads, dim]'}, got {tuple(t.shape)}")
+    if t.stride(2) != 1 and t.shape[2] != 1:
+        raise ValueError(f"{name}: the elements of a head must be adjacent (strides {t.stride()})")
+    return t
+
+
+def _on_device(*tensors) -> torch.cuda.device:
+    """the device that the tensors share, as a context: launches and the current stream are its own, whichever device is current"""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}: one device is wanted")
+    return torch.cuda.device(dev)
+
+
+def _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale) -> N.AttnGqaArgs:
+    _rows3(q, "q")
+    T, heads, dim = q.shape
+    _rows3(k, "k")
+    kv_heads = k.shape[1]
+    _rows3(k, "k", (T, kv_heads, dim))
+    _rows3(v, "v", (T, kv_heads, dim))
+    _req(seq_off, I32, "seq_off", 1)
+    if T < 1 or seq_off.shape[0] < 2:
+        raise ValueError(f"attn_gqa: {T} rows, seq_off of {seq_off.shape[0]}: at least one row and one sequence (B + 1 offsets) are wanted")
+    if mask is not None:
+        _req(mask, I32, "mask", 1)
+        if mask.shape[0] != T:
+            raise ValueError(f"attn_gqa: mask of {mask.shape[0]} entries for {T} rows")
+    left, right = (int(w) for w in window)
+    if causal:
+        if right > 0:
+            raise ValueError(f"attn_gqa: causal rows see nothing to their right (window {tuple(window)})")
+        right = 0
+    scale = dim ** -0.5 if scale is None else float(scale)
+    return N.AttnGqaArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), seq_off.data_ptr(), 0 if mask is None else mask.data_ptr(),
+                         q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
+                         T, seq_off.shape[0] - 1, heads, kv_heads, dim, left, right, scale)
+
+
+def attn_gqa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: torch.Tensor, *, causal: bool = False,
+                 window: Tuple[int, int] = (-1, -1), mask: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                 out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(ctx [T, heads, dim] bf16, lse [heads, T] fp32): softmax(scale q k^T) v of every packed sequence, see cocodr_attn_gqa_fwd.
+
+    q [T, heads, dim], k / v [T, kv_heads, dim] bf16, any strides that are multiples of 8 with the elements of a head adjacent (views of
+    a fused projection output); heads a multiple of kv_heads; dim a multiple of 8 up to 128; seq_off int32 [B + 1]; mask int32 [T], 0 =
+    the key is not seen; window (left, right) = how many rows before and behind its own a query sees (-1: all); scale: 1 / sqrt(dim)
+    unless given.  A row that sees nothing gets ctx 0 and lse -inf, and so do the rows of no sequence - unless ``out`` is given: there
+    they are left as they are (their lse is unspecified)."""
+    a = _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale)
+    with _on_device(q, k, v, seq_off, mask, out):
+        ctx = torch.empty(q.shape, dtype=BF16, device=q.device) if out is None else _rows3(out, "out", tuple(q.shape))
+        lse = torch.empty((a.heads, a.T), dtype=F32, device=q.device)
+        a.o_row, a.o_head = ctx.stride(0), ctx.stride(1)
+        check(lib().cocodr_attn_gqa_fwd(C.byref(a), ptr(ctx), ptr(lse), int(out is None), stream_ptr()), "attn_gqa_fwd")
+    return ctx, lse
+
+
+def attn_gqa_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: torch.Tensor, dctx: torch.Tensor, lse: torch.Tensor,
+                 seq_off: torch.Tensor, *, causal: bool = False, window: Tuple[int, int] = (-1, -1), mask: Optional[torch.Tensor] = None,
+                 scale: Optional[float] = None, out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
+    """(dq [T, heads, dim], dk, dv [T, kv_heads, dim]) bf16 of attn_gqa_fwd with the same q .. scale, its ctx and lse, and the gradient
+    dctx of ctx (ctx and dctx with any strides as q's; they need not be the same).  The rows of no sequence get zeros; with ``out`` (three
+    tensors to write to, e.g. views of one fused gradient) they are left as they are.  Deterministic."""
+    a = _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale)
+    _rows3(ctx, "ctx", tuple(q.shape)); _rows3(dctx, "dctx", tuple(q.shape)); _req(lse, F32, "lse", 2)
+    if tuple(lse.shape) != (a.heads, a.T):
+        raise ValueError(f"attn_gqa_bwd: lse {tuple(lse.shape)} is not [heads, T] = {(a.heads, a.T)}")
+    if out is not None and len(out) != 3:
+        raise ValueError("attn_gqa_bwd: out holds dq, dk and dv")
+    with _on_device(q, k, v, seq_off, mask, ctx, dctx, lse, *(out or ())):
+        if out is None:
+            dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
+        else:
+            dq, dk, dv = (_rows3(t, n, tuple(x.shape)) for t, n, x in zip(out, ("dq", "dk", "dv"), (q, k, v)))
+        a.o_row, a.o_head, a.do_row, a.do_head = ctx.stride(0), ctx.stride(1), dctx.stride(0), dctx.stride(1)
+        a.dq_row, a.dq_head, a.dk_row, a.dk_head, a.dv_row, a.dv_head = (dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1), dv.stride(0), dv.stride(1))
+        floats = lib().cocodr_attn_gqa_bwd_workspace_floats(C.byref(a))
+        ws = torch.empty(floats, dtype=F32, device=q.device)
+        check(lib().cocodr_attn_gqa_bwd(C.byref(a), ptr(ctx), ptr(dctx), ptr(lse), ptr(dq), ptr(dk), ptr(dv), int(out is None), ptr(ws), floats,
+                                        stream_ptr()), "attn_gqa_bwd")
+    return dq, dk, dv
+
+
 # ----------------------------------------------------------------------------------------------- row kernels
 def embed_ln_fwd(ids, word, pos, type0, gamma, beta, eps: float = 1e-12, drop: Optional[N.DropoutMask] = None):
     _req(ids, I32, "ids", 2)

@@ -171,6 +171,37 @@ int cocodr_attn_bwd_drop(const uint16_t* qkv, const int32_t* mask, const uint16_
                          const cocodr_dropout_mask* drop, cocodr_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Attention over packed sequences with grouped heads: decoder and long-document backbones (any length, head sizes up to 128,
+ * causal or within a window).  q is [T, heads, dim], k and v are [T, kv_heads, dim] bf16 with the strides given (elements;
+ * *_row from token to token, *_head from head to head, the dim elements of a head adjacent) - e.g. three views of one fused
+ * projection output.  Query head h reads key head h / (heads / kv_heads).  Sequence b is the rows seq_off[b] .. seq_off[b+1]-1
+ * (int32 [B+1] on the device, not decreasing; values outside [0, T] are cut to it; a sequence may be empty).  Query i of a sequence
+ * sees its keys j with i - left <= j <= i + right (-1: no limit; causal = right 0) whose mask entry (int32 [T], NULL: all) is not 0.
+ *   ctx_i = sum_j softmax_j(scale q_i . k_j) v_j [T, heads, dim] bf16, lse [heads, T] fp32 = log sum_j exp(scale q_i . k_j);
+ *   a row that sees nothing gets ctx = 0, lse = -inf and zero gradients.  K and V rows behind a sequence or masked out are not read
+ *   (they may hold anything, NaN too).
+ * fill: rows that belong to no sequence get ctx = 0 and lse = -inf, zero gradients (1), or are left as they are (0).
+ * Backward: recomputes the probabilities from q, k and lse; dk and dv sum over the query heads of a key head's group.  No atomics:
+ * the same inputs give the same bits.  workspace: cocodr_attn_gqa_bwd_workspace_floats(args) floats.
+ * Requirements: dim % 8 == 0, dim <= 128; pointers (not lse, seq_off, mask) 16-byte aligned; strides multiples of 8, rows less than
+ * 2^23 elements apart; rows and heads of an output do not overlap; scale > 0; T < 2^30.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct {
+  const uint16_t *q, *k, *v;
+  const int32_t* seq_off;
+  const int32_t* mask; /* or NULL */
+  long long q_row, q_head, k_row, k_head, v_row, v_head;
+  long long o_row, o_head, do_row, do_head;                        /* ctx, dctx */
+  long long dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;     /* backward only */
+  int T, B, heads, kv_heads, dim, left, right;
+  float scale;
+} cocodr_attn_gqa_args;
+int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* args, uint16_t* ctx, float* lse, int fill, cocodr_stream_t stream);
+size_t cocodr_attn_gqa_bwd_workspace_floats(const cocodr_attn_gqa_args* args);
+int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* args, const uint16_t* ctx, const uint16_t* dctx, const float* lse, uint16_t* dq,
+                        uint16_t* dk, uint16_t* dv, int fill, float* workspace, size_t workspace_floats, cocodr_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Row kernels (HBM bound)
  * embed_ln: hf BertEmbeddings.forward :68-108 - LN(word[ids] + pos[0..L-1] + type[0]), eps 1e-12;
  *           the reference never passes token_type_ids / position_ids (COCO/data.py:140,
