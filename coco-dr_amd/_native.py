@@ -126,6 +126,11 @@ SIGNATURES = {
     "cocodr_attn_gqa_fwd": (c_int, [C.POINTER(AttnGqaArgs), c_void_p, c_void_p, c_int, c_void_p]),
     "cocodr_attn_gqa_bwd_workspace_floats": (c_size_t, [C.POINTER(AttnGqaArgs)]),
     "cocodr_attn_gqa_bwd": (c_int, [C.POINTER(AttnGqaArgs)] + [c_void_p] * 6 + [c_int, c_void_p, c_size_t, c_void_p]),
+    "cocodr_embed_fwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_float, c_void_p]),
+    "cocodr_embed_bwd_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "cocodr_embed_bwd": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_float, c_int, c_void_p, c_size_t, c_void_p]),
+    "cocodr_dropout_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_int, C.POINTER(DropoutMask), c_void_p]),
+    "cocodr_dropout_bwd": (c_int, [c_void_p, c_void_p, c_size_t, c_int, C.POINTER(DropoutMask), c_void_p]),
     "cocodr_embed_ln_fwd": (c_int, [c_void_p] * 9 + [c_int, c_int, c_int, c_int, c_float, c_void_p]),
     "cocodr_embed_bwd_partial_floats": (c_size_t, [c_int, c_int]),
     "cocodr_embed_ln_bwd": (c_int, [c_void_p] * 14 + [c_int, c_int, c_int, c_int, c_void_p]),

@@ -12,10 +12,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libcocodr_hip.so")
-SOURCES = ["core.hip", "gemm.hip", "gemm_pp.hip", "gemm_a4.hip", "attention.hip", "attn_gqa.hip", "rowops.hip", "loss.hip", "score.hip", "merge.hip", "encoder.hip", "collate.hip", "probe.hip", "comm.hip"]
+SOURCES = ["core.hip", "gemm.hip", "gemm_pp.hip", "gemm_a4.hip", "attention.hip", "attn_gqa.hip", "rowops.hip", "embed.hip", "dropout.hip", "loss.hip", "score.hip", "merge.hip", "encoder.hip", "collate.hip", "probe.hip", "comm.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-result", "-Wno-unused-value"]
 # no v_pk_{add,mul,fma}_f32 in the sources named here (the host pass of hipcc warns that it does not know the feature: harmless)
-SCALAR_F32 = {"attn_gqa.hip"}
+SCALAR_F32 = {"attn_gqa.hip", "embed.hip", "dropout.hip"}
 SCALAR_F32_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 FLAGS += os.environ.get("COCODR_EXTRA_FLAGS", "").split()  # measurement builds only (tools/gemm_ablate.py: -DCOCODR_ABL_*)
 

@@ -268,6 +268,75 @@ def attn_gqa_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: torch.T
     return dq, dk, dv
 
 
+# ----------------------------------------------------------------------------------------------- embedding, dropout
+def _req_any(t: torch.Tensor, dtypes, name: str, dims: Optional[int] = None) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype not in dtypes:
+        raise ValueError(f"{name}: expected dtype {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    return _req(t, t.dtype if isinstance(t, torch.Tensor) else None, name, dims)
+
+
+def embed_fwd(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out_dtype: torch.dtype = BF16) -> torch.Tensor:
+    """scale * table[ids]: ids int32 / int64 of any shape, table [vocab, H] fp32 or bf16, the result ids.shape + [H] bf16 or fp32 (one
+    rounding).  An id outside [0, vocab) is padding: a row of zeros.  H % 8 == 0."""
+    _req_any(ids, (I32, I64), "ids"); _req_any(table, (F32, BF16), "table", 2)
+    if out_dtype not in (F32, BF16):
+        raise ValueError(f"embed_fwd: out_dtype {out_dtype}: {F32} or {BF16} is wanted")
+    V, H = table.shape
+    with _on_device(table, ids):
+        out = torch.empty(tuple(ids.shape) + (H,), dtype=out_dtype, device=table.device)
+        check(lib().cocodr_embed_fwd(ptr(ids), int(ids.dtype == I64), ptr(table), int(table.dtype == F32), ptr(out), int(out_dtype == F32),
+                                     ids.numel(), H, V, float(scale), stream_ptr()), "embed_fwd")
+    return out
+
+
+def embed_bwd(dout: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
+              accumulate: bool = False) -> torch.Tensor:
+    """The gradient [vocab, H] fp32 of embed_fwd's table: scale * the sum of dout's rows (bf16 or fp32, ids.shape + [H]) of each id, summed
+    in the order of the tokens (deterministic: no float atomics); zero rows for ids that do not occur.  ``out`` receives it; with
+    ``accumulate`` it is added to what ``out`` holds (rows of other ids are not touched)."""
+    _req_any(dout, (F32, BF16), "dout"); _req_any(ids, (I32, I64), "ids")
+    if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
+        raise ValueError(f"embed_bwd: dout {tuple(dout.shape)} is not ids {tuple(ids.shape)} + [H]")
+    H, V = dout.shape[-1], int(vocab)
+    if accumulate and out is None:
+        raise ValueError("embed_bwd: accumulate needs the tensor to add to (out)")
+    if out is not None:
+        _req(out, F32, "out", 2)
+        if tuple(out.shape) != (V, H):
+            raise ValueError(f"embed_bwd: out {tuple(out.shape)} is not [vocab, H] = {(V, H)}")
+    with _on_device(dout, ids, out):
+        if out is None:
+            out = torch.empty((V, H), dtype=F32, device=dout.device)
+        n = ids.numel()
+        ws = torch.empty(lib().cocodr_embed_bwd_workspace_bytes(n, H, V), dtype=torch.uint8, device=dout.device)
+        check(lib().cocodr_embed_bwd(ptr(dout), int(dout.dtype == F32), ptr(ids), int(ids.dtype == I64), ptr(out), n, H, V, float(scale),
+                                     int(bool(accumulate)), ptr(ws), ws.numel(), stream_ptr()), "embed_bwd")
+    return out
+
+
+def dropout_fwd(x: torch.Tensor, drop: N.DropoutMask, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dropout(x) (+ residual) with the keys of ``drop`` (dropout_mask) over x's flat index; bf16 or fp32, any shape, one rounding.  The
+    mask is not stored: dropout_bwd with the same ``drop`` makes it again."""
+    _req_any(x, (F32, BF16), "x")
+    if residual is not None:
+        _req(residual, x.dtype, "residual")
+        if residual.shape != x.shape:
+            raise ValueError(f"dropout_fwd: residual {tuple(residual.shape)} is not x's shape {tuple(x.shape)}")
+    with _on_device(x, residual):
+        out = torch.empty_like(x)
+        check(lib().cocodr_dropout_fwd(ptr(x), ptr(residual), ptr(out), x.numel(), int(x.dtype == F32), C.byref(drop), stream_ptr()), "dropout_fwd")
+    return out
+
+
+def dropout_bwd(dout: torch.Tensor, drop: N.DropoutMask) -> torch.Tensor:
+    """The gradient of dropout_fwd's x (that of its residual is dout itself)."""
+    _req_any(dout, (F32, BF16), "dout")
+    with _on_device(dout):
+        dx = torch.empty_like(dout)
+        check(lib().cocodr_dropout_bwd(ptr(dout), ptr(dx), dout.numel(), int(dout.dtype == F32), C.byref(drop), stream_ptr()), "dropout_bwd")
+    return dx
+
+
 # ----------------------------------------------------------------------------------------------- row kernels
 def embed_ln_fwd(ids, word, pos, type0, gamma, beta, eps: float = 1e-12, drop: Optional[N.DropoutMask] = None):
     _req(ids, I32, "ids", 2)

@@ -266,6 +266,24 @@ int cocodr_cls_rows(const int32_t* seq_off, int L, int B, long long* idx, cocodr
 /* d_last[b*L + 0, :] = bf16(dE[b, :]), all other rows zero (gradient enters at [CLS] only) */
 int cocodr_scatter_cls_grad(const float* dE, uint16_t* d_last, int B, int L, int H, cocodr_stream_t stream);
 
+/* Embedding lookup with scaling: out[t] = scale * table[ids[t]] (rows of H; bf16 or fp32 each, *_f32 != 0: fp32), and its gradient
+ * dtable[v] = scale * sum over ids[t] == v of dout[t] (fp32 [vocab, H], all rows written; accumulate != 0: added to what is there), e.g.
+ * the token embedding of a decoder backbone, scaled by sqrt(H) in some.  ids int32 or int64 (ids_i64 != 0) [n]; an id outside
+ * [0, vocab) is padding: a zero row, no gradient.  The gradient's sums run in the order of the tokens, without float atomics: the same
+ * inputs give the same bits.  H % 8 == 0; tensors 16-byte aligned; workspace: cocodr_embed_bwd_workspace_bytes(n, H, vocab) bytes,
+ * 16-byte aligned. */
+int cocodr_embed_fwd(const void* ids, int ids_i64, const void* table, int table_f32, void* out, int out_f32, int n, int H, int vocab,
+                     float scale, cocodr_stream_t stream);
+size_t cocodr_embed_bwd_workspace_bytes(int n, int H, int vocab);
+int cocodr_embed_bwd(const void* dout, int dout_f32, const void* ids, int ids_i64, float* dtable, int n, int H, int vocab, float scale,
+                     int accumulate, void* workspace, size_t workspace_bytes, cocodr_stream_t stream);
+/* Dropout as an operator of its own, with the mask of "Dropout" above over the flat index of x: out = dropout(x) (+ residual, or NULL)
+ * and dx = dropout(dout) with the same keys; bf16 or fp32 (f32 != 0) [n], n <= 2^33 (the generator counts 2^32 pairs).  out / dx may be
+ * x / dout / residual themselves. */
+int cocodr_dropout_fwd(const void* x, const void* residual, void* out, size_t n, int f32, const cocodr_dropout_mask* drop,
+                       cocodr_stream_t stream);
+int cocodr_dropout_bwd(const void* dout, void* dx, size_t n, int f32, const cocodr_dropout_mask* drop, cocodr_stream_t stream);
+
 /* Fused AdamW over one flat fp32 parameter (torch.optim.AdamW semantics; the reference steps AdamW through the HF
  * Trainer, COCO/trainer.py:66-70, or its own loop, ANCE/drivers/run_ann.py:345-356).  g is multiplied by grad_scale
  * (and by *grad_scale_dev when that device pointer is not NULL - the clip coefficient below) first.  When
