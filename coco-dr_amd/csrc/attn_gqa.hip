@@ -269,36 +269,12 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// -delta and -lse (in log2 units) of every row and query head, [heads][T] each.  16 lanes share a row.
-__global__ __launch_bounds__(256) void attn_gqa_delta_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,
-                                                             const float* __restrict__ lse, float* __restrict__ ndelta, float* __restrict__ nlse) {
-  const int lane = threadIdx.x & 15;
-  const long long i = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (i >= (long long)a.T * a.heads) return;
-  const int row = (int)(i / a.heads), h = (int)(i % a.heads);
-  float sum = 0.f;
-  if (lane * 8 < a.dim) {
-    float x[8], y[8];
-    unpack8(*reinterpret_cast<const uint4*>(ctx + row * a.o_row + h * a.o_head + lane * 8), x);
-    unpack8(*reinterpret_cast<const uint4*>(dctx + row * a.do_row + h * a.do_head + lane * 8), y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(x[e], y[e], sum);
-  }
-  sum += dpp_partner<0xB1>(sum);
-  sum += dpp_partner<0x4E>(sum);
-  sum += dpp_partner<0x141>(sum);
-  sum += dpp_partner<0x140>(sum);
-  if (lane == 0) {
-    const size_t at = (size_t)h * a.T + row;
-    ndelta[at] = -sum;
-    nlse[at] = -lse[at] * kLog2e;
-  }
-}
-
-// dQ: 128 query rows of one head a workgroup, 32 a wave (lane = query), over tiles of 64 keys as in the forward
+// dQ: 128 query rows of one head a workgroup, 32 a wave (lane = query), over tiles of 64 keys as in the forward.  A wave has its rows of dO in
+// registers: with ctx beside them it also makes -delta and -lse (in log2 units) of its rows and leaves them, [heads][T] each, for the dK / dV kernel.
 template <int DP>
-__global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
-                                                             const float* __restrict__ nlse, uint16_t* __restrict__ dq, int fill) {
+__global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,
+                                                             const float* __restrict__ lse, float* __restrict__ ndelta, float* __restrict__ nlse,
+                                                             uint16_t* __restrict__ dq, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) {
@@ -322,7 +298,25 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
   load_frags<DP>(df, dctx + (long long)(tile.row0 + qi) * a.do_row + h * a.do_head, a.dim, qi < n, half);
   const size_t at = (size_t)h * a.T + tile.row0 + qi;
-  const float nd = qi < n ? ndelta[at] : 0.f, nl = qi < n ? nlse[at] : 0.f;
+  const float nl = qi < n ? -lse[at] * kLog2e : 0.f;
+  float nd = 0.f;
+  {
+    bf16x8 of[DP / 16];
+    load_frags<DP>(of, ctx + (long long)(tile.row0 + qi) * a.o_row + h * a.o_head, a.dim, qi < n, half);
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      float x[8], y[8];
+      unpack8(__builtin_bit_cast(uint4, of[c]), x);
+      unpack8(__builtin_bit_cast(uint4, df[c]), y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) nd = fmaf(-x[e], y[e], nd);
+    }
+    nd += __shfl_xor(nd, 32, 64);
+  }
+  if (qi < n && lane < 32) {
+    ndelta[at] = nd;
+    nlse[at] = nl;
+  }
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -387,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
 
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows
 template <int DP>
-__global__ __launch_bounds__(256, 1) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
+__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
                                                               int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -521,7 +515,7 @@ int check(const Args* a, const char* what) {
   CK_ARG(aligned16(a->q) && aligned16(a->k) && aligned16(a->v), "%s: q, k, v must be 16-byte aligned", what);
   CK_ARG(stride_ok(a->q_row, a->q_head, a->T, a->heads) && stride_ok(a->k_row, a->k_head, a->T, a->kv_heads) && stride_ok(a->v_row, a->v_head, a->T, a->kv_heads), "%s: strides must be multiples of 8 elements, rows less than 2^23 apart", what);
   const long long units = ((long long)a->T / 128 + a->B) * a->heads;
-  CK_ARG(units <= INT_MAX && (long long)a->T * a->heads / 16 < INT_MAX, "%s: too many rows and heads for one launch", what);
+  CK_ARG(units <= INT_MAX, "%s: too many rows and heads for one launch", what);
   return COCODR_OK;
 }
 
@@ -570,15 +564,13 @@ extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t
   lds_limits();
   hipStream_t st = (hipStream_t)stream;
   float *ndelta = workspace, *nlse = workspace + (size_t)a->T * a->heads;
-  hipLaunchKernelGGL(attn_gqa_delta_kernel, dim3((unsigned)(((long long)a->T * a->heads + 15) / 16)), dim3(256), 0, st, *a, ctx, dctx, lse, ndelta, nlse);
-  CK_LAUNCH("attn_gqa_delta");
   const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)((a->T / 128 + a->B) * a->kv_heads));
   if (a->dim <= 64) {
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, fill);
     hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, fill);
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, dctx, ndelta, nlse, dq, fill);
   } else {
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, fill);
     hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, fill);
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, dctx, ndelta, nlse, dq, fill);
   }
   CK_LAUNCH("attn_gqa_bwd");
   return COCODR_OK;

@@ -7,58 +7,57 @@
 
 namespace {
 
-constexpr int kPer = 8;  // elements a thread takes at once: 16 bytes of bf16, twice 16 of fp32
+// elements a thread takes at once: 16 bytes, so that a wave's access is whole lines
+template <bool F32> constexpr int kPer = F32 ? 4 : 8;
 
 template <bool F32> struct Elem;
 template <> struct Elem<false> {
   typedef uint16_t T;
-  static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), v); }
-  static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) { *reinterpret_cast<uint4*>(p) = pack8(v); }
+  static __device__ __forceinline__ void load(const T* p, float (&v)[8]) { unpack8(*reinterpret_cast<const uint4*>(p), v); }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[8]) { *reinterpret_cast<uint4*>(p) = pack8(v); }
   static __device__ __forceinline__ float load(const T* p) { return bf2f(*p); }
   static __device__ __forceinline__ void store(T* p, float v) { *p = f2bf(v); }
 };
 template <> struct Elem<true> {
   typedef float T;
-  static __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  static __device__ __forceinline__ void load(const T* p, float (&v)[4]) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   }
-  static __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
+  static __device__ __forceinline__ void store(T* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
   static __device__ __forceinline__ float load(const T* p) { return *p; }
   static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
 };
 
-// WIDE: all pointers are 16-byte aligned (a contiguous view into a larger tensor may begin anywhere); the last n % 8 elements go one by one
+// WIDE: all pointers are 16-byte aligned (a contiguous view into a larger tensor may begin anywhere); what is left of n goes one by one
 template <bool F32, bool ADD, bool WIDE>
 __global__ __launch_bounds__(256) void dropout_kernel(const void* x_, const void* r_, void* out_, size_t n, const cocodr_dropout_mask dm) {
   typedef Elem<F32> E;
   const typename E::T *x = (const typename E::T*)x_, *r = (const typename E::T*)r_;
   typename E::T* out = (typename E::T*)out_;
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * kPer; i < n; i += (size_t)gridDim.x * 256 * kPer) {
-    float v[8], w[8];
-    const bool whole = i + kPer <= n;
+  constexpr int PER = kPer<F32>;
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * PER; i < n; i += (size_t)gridDim.x * 256 * PER) {
+    float v[PER], w[PER];
+    const bool whole = i + PER <= n;
     if (WIDE && whole) {
-      E::load8(x + i, v);
-      if constexpr (ADD) E::load8(r + i, w);
+      E::load(x + i, v);
+      if constexpr (ADD) E::load(r + i, w);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < PER; ++e) {
         v[e] = i + e < n ? E::load(x + i + e) : 0.f;
         if constexpr (ADD) w[e] = i + e < n ? E::load(r + i + e) : 0.f;
       }
     }
-    drop_apply<8>(v, i, dm);
+    drop_apply<PER>(v, i, dm);
     if constexpr (ADD) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] += w[e];
+      for (int e = 0; e < PER; ++e) v[e] += w[e];
     }
-    if (WIDE && whole) E::store8(out + i, v);
+    if (WIDE && whole) E::store(out + i, v);
     else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < PER; ++e)
         if (i + e < n) E::store(out + i + e, v[e]);
     }
   }
@@ -67,7 +66,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const void* x_, const void
 template <bool F32, bool ADD>
 void launch(const void* x, const void* r, void* out, size_t n, const cocodr_dropout_mask& dm, hipStream_t st) {
   const bool wide = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(r) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const size_t groups = (n + 256 * kPer - 1) / (256 * kPer);
+  const size_t groups = (n + 256 * kPer<F32> - 1) / (256 * kPer<F32>);
   const dim3 grid((unsigned)(groups < 65536 ? groups : 65536));
   if (wide) hipLaunchKernelGGL((dropout_kernel<F32, ADD, true>), grid, dim3(256), 0, st, x, r, out, n, dm);
   else hipLaunchKernelGGL((dropout_kernel<F32, ADD, false>), grid, dim3(256), 0, st, x, r, out, n, dm);

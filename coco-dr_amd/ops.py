@@ -3,6 +3,7 @@ memory and the current stream only; all arithmetic happens in libcocodr_hip.so. 
 contiguity problems raise ValueError here, mirroring where ATen would raise for the reference."""
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 from typing import Optional, Tuple
 
@@ -189,13 +190,25 @@ def _rows3(t: torch.Tensor, name: str, shape=None) -> torch.Tensor:
     return t
 
 
-def _on_device(*tensors) -> torch.cuda.device:
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(*tensors):
     """the device that the tensors share, as a context: launches and the current stream are its own, whichever device is current"""
     dev = tensors[0].device
     for t in tensors:
         if t is not None and t.device != dev:
             raise ValueError(f"tensors on {dev} and {t.device}: one device is wanted")
-    return torch.cuda.device(dev)
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(t: torch.Tensor) -> int:
+    """the current stream of t's device, as a handle (torch.cuda.current_stream builds a Python object on the way: 5 us of a 13 us call)"""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale) -> N.AttnGqaArgs:
@@ -218,9 +231,9 @@ def _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale) -> N.AttnGqaAr
             raise ValueError(f"attn_gqa: causal rows see nothing to their right (window {tuple(window)})")
         right = 0
     scale = dim ** -0.5 if scale is None else float(scale)
-    return N.AttnGqaArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), seq_off.data_ptr(), 0 if mask is None else mask.data_ptr(),
-                         q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0,
-                         T, seq_off.shape[0] - 1, heads, kv_heads, dim, left, right, scale)
+    (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
+    return N.AttnGqaArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), seq_off.data_ptr(), _addr(mask), q0, q1, k0, k1, v0, v1,
+                         0, 0, 0, 0, 0, 0, 0, 0, 0, 0, T, seq_off.shape[0] - 1, heads, kv_heads, dim, left, right, scale)
 
 
 def attn_gqa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: torch.Tensor, *, causal: bool = False,
@@ -237,8 +250,8 @@ def attn_gqa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: tor
     with _on_device(q, k, v, seq_off, mask, out):
         ctx = torch.empty(q.shape, dtype=BF16, device=q.device) if out is None else _rows3(out, "out", tuple(q.shape))
         lse = torch.empty((a.heads, a.T), dtype=F32, device=q.device)
-        a.o_row, a.o_head = ctx.stride(0), ctx.stride(1)
-        check(lib().cocodr_attn_gqa_fwd(C.byref(a), ptr(ctx), ptr(lse), int(out is None), stream_ptr()), "attn_gqa_fwd")
+        a.o_row, a.o_head, _ = ctx.stride()
+        check(lib().cocodr_attn_gqa_fwd(C.byref(a), _addr(ctx), _addr(lse), int(out is None), _stream(q)), "attn_gqa_fwd")
     return ctx, lse
 
 
@@ -259,12 +272,12 @@ def attn_gqa_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: torch.T
             dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
         else:
             dq, dk, dv = (_rows3(t, n, tuple(x.shape)) for t, n, x in zip(out, ("dq", "dk", "dv"), (q, k, v)))
-        a.o_row, a.o_head, a.do_row, a.do_head = ctx.stride(0), ctx.stride(1), dctx.stride(0), dctx.stride(1)
-        a.dq_row, a.dq_head, a.dk_row, a.dk_head, a.dv_row, a.dv_head = (dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1), dv.stride(0), dv.stride(1))
+        (a.o_row, a.o_head, _), (a.do_row, a.do_head, _) = ctx.stride(), dctx.stride()
+        (a.dq_row, a.dq_head, _), (a.dk_row, a.dk_head, _), (a.dv_row, a.dv_head, _) = dq.stride(), dk.stride(), dv.stride()
         floats = lib().cocodr_attn_gqa_bwd_workspace_floats(C.byref(a))
         ws = torch.empty(floats, dtype=F32, device=q.device)
-        check(lib().cocodr_attn_gqa_bwd(C.byref(a), ptr(ctx), ptr(dctx), ptr(lse), ptr(dq), ptr(dk), ptr(dv), int(out is None), ptr(ws), floats,
-                                        stream_ptr()), "attn_gqa_bwd")
+        check(lib().cocodr_attn_gqa_bwd(C.byref(a), _addr(ctx), _addr(dctx), _addr(lse), _addr(dq), _addr(dk), _addr(dv), int(out is None), _addr(ws), floats,
+                                        _stream(q)), "attn_gqa_bwd")
     return dq, dk, dv
 
 
@@ -284,8 +297,8 @@ def embed_fwd(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out
     V, H = table.shape
     with _on_device(table, ids):
         out = torch.empty(tuple(ids.shape) + (H,), dtype=out_dtype, device=table.device)
-        check(lib().cocodr_embed_fwd(ptr(ids), int(ids.dtype == I64), ptr(table), int(table.dtype == F32), ptr(out), int(out_dtype == F32),
-                                     ids.numel(), H, V, float(scale), stream_ptr()), "embed_fwd")
+        check(lib().cocodr_embed_fwd(_addr(ids), int(ids.dtype == I64), _addr(table), int(table.dtype == F32), _addr(out), int(out_dtype == F32),
+                                     ids.numel(), H, V, float(scale), _stream(table)), "embed_fwd")
     return out
 
 
@@ -309,8 +322,8 @@ def embed_bwd(dout: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float
             out = torch.empty((V, H), dtype=F32, device=dout.device)
         n = ids.numel()
         ws = torch.empty(lib().cocodr_embed_bwd_workspace_bytes(n, H, V), dtype=torch.uint8, device=dout.device)
-        check(lib().cocodr_embed_bwd(ptr(dout), int(dout.dtype == F32), ptr(ids), int(ids.dtype == I64), ptr(out), n, H, V, float(scale),
-                                     int(bool(accumulate)), ptr(ws), ws.numel(), stream_ptr()), "embed_bwd")
+        check(lib().cocodr_embed_bwd(_addr(dout), int(dout.dtype == F32), _addr(ids), int(ids.dtype == I64), _addr(out), n, H, V, float(scale),
+                                     int(bool(accumulate)), _addr(ws), ws.numel(), _stream(dout)), "embed_bwd")
     return out
 
 
@@ -324,7 +337,7 @@ def dropout_fwd(x: torch.Tensor, drop: N.DropoutMask, residual: Optional[torch.T
             raise ValueError(f"dropout_fwd: residual {tuple(residual.shape)} is not x's shape {tuple(x.shape)}")
     with _on_device(x, residual):
         out = torch.empty_like(x)
-        check(lib().cocodr_dropout_fwd(ptr(x), ptr(residual), ptr(out), x.numel(), int(x.dtype == F32), C.byref(drop), stream_ptr()), "dropout_fwd")
+        check(lib().cocodr_dropout_fwd(_addr(x), _addr(residual), _addr(out), x.numel(), int(x.dtype == F32), C.byref(drop), _stream(x)), "dropout_fwd")
     return out
 
 
@@ -333,7 +346,7 @@ def dropout_bwd(dout: torch.Tensor, drop: N.DropoutMask) -> torch.Tensor:
     _req_any(dout, (F32, BF16), "dout")
     with _on_device(dout):
         dx = torch.empty_like(dout)
-        check(lib().cocodr_dropout_bwd(ptr(dout), ptr(dx), dout.numel(), int(dout.dtype == F32), C.byref(drop), stream_ptr()), "dropout_bwd")
+        check(lib().cocodr_dropout_bwd(_addr(dout), _addr(dx), dout.numel(), int(dout.dtype == F32), C.byref(drop), _stream(dout)), "dropout_bwd")
     return dx
 
 

@@ -41,7 +41,7 @@ def test_embed_fwd(n, V, H, idt, table, out):
     assert torch.equal(ops.embed_fwd(ids.view(1, n, 1), E, scale=27.7128, out_dtype=out).view(n, H), got)
 
 
-BWD = [("text", 1, 1, 8), ("text", 64, 3, 64), ("one", 64, 4, 768), ("one", 65, 4, 768), ("one", 5000, 10, 520), ("one", 40000, 9, 64), ("two", 9000, 1025, 1032),
+BWD = [("text", 1, 1, 8), ("one", 1, 2, 8), ("one", 3, 9, 8), ("text", 64, 3, 64), ("one", 64, 4, 768), ("one", 65, 4, 768), ("one", 5000, 10, 520), ("one", 40000, 9, 64), ("two", 9000, 1025, 1032),
        ("text", 8192, 30522, 768), ("pads", 777, 40, 40), ("pads", 20000, 100, 16), ("distinct", 4096, 5000, 128), ("text", 33333, 2000, 264), ("two", 140000, 2, 8)]
 
 
