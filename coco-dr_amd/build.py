@@ -17,9 +17,6 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-res
 # no v_pk_{add,mul,fma}_f32 in the sources named here (the host pass of hipcc warns that it does not know the feature: harmless)
 SCALAR_F32 = {"attn_gqa.hip", "embed.hip", "dropout.hip"}
 SCALAR_F32_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# accumulators of the matrix pipe in VGPRs unless the source says otherwise: with 512 registers a wave hipcc puts all of them in AGPRs and copies
-# those that vector instructions read
-SOURCE_FLAGS = {"attn_gqa.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 FLAGS += os.environ.get("COCODR_EXTRA_FLAGS", "").split()  # measurement builds only (tools/gemm_ablate.py: -DCOCODR_ABL_*)
 
 
@@ -51,7 +48,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(job):
         s, o = job
-        cmd = [hipcc] + FLAGS + (SCALAR_F32_FLAGS if os.path.basename(s) in SCALAR_F32 else []) + SOURCE_FLAGS.get(os.path.basename(s), []) + ["-c", s, "-o", o]
+        cmd = [hipcc] + FLAGS + (SCALAR_F32_FLAGS if os.path.basename(s) in SCALAR_F32 else []) + ["-c", s, "-o", o]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed for %s:\n%s" % (s, r.stderr[-4000:]))

@@ -31,6 +31,15 @@ constexpr int BK = 64;          // rows of a staged tile
 
 typedef cocodr_attn_gqa_args Args;
 
+// f(0), f(1), .. f(N - 1) with the index as a constant
+template <int N, class F> __device__ __forceinline__ void each(F&& f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+#define SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
+
 // ------------------------------------------------------------------------------------------------ tiles in LDS
 // [rows][DP] bf16, DP = 64 or 128 (the head size rounded up; columns behind it are zeros).  The 16-byte chunks of a row are permuted
 // so that both reads are free of bank conflicts: ds_read_b128 of 16 consecutive rows at one chunk, and the transposing read of 4
@@ -75,34 +84,45 @@ __device__ __forceinline__ void dma4(rsrc_t rs, uint32_t off, uint32_t dst) {
 // this wave's transfers are in LDS; with the barrier behind it, every wave's
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// the lane's number, made where it is used: kept in a register, or what is derived from it, it is one too many in the kernels that use them all
+__device__ __forceinline__ int fresh_lane() {
+  int l = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  asm volatile("" : "+v"(l));
+  return l;
+}
+
 // BK rows of one head into a tile by LDS DMA: a wave's instruction (a piece) writes 1 KiB lane-linear, so the permutation goes into the source
 // addresses.  Rows whose bit of `rows` is 0 (behind the sequence, masked out) and columns >= D are addressed behind the descriptor's
 // end and arrive as zeros: whatever stands there in memory, NaN too, is not read.  The descriptor reaches over one tile only, so its
-// 32-bit offsets do for any buffer.  Wave w has the pieces w, w + 4, ..: the permutation of its rows is the same in each, and a piece's
+// 32-bit offsets do for any buffer.  Wave w of 4 has the pieces w, w + 4, ..: the permutation of its rows is the same in each, and a piece's
 // offset differs from the first's by a scalar.
 template <int DP> struct Stager {
   static constexpr int CH = DP / 8, RP = 64 / CH, PIECES = BK / RP / 4;  // chunks of a row, rows of a piece, pieces of a wave
   uint32_t ldb, span, first;  // bytes of a row, of a tile; this lane's offset in its wave's first piece
-  int row;                    // the lane's row in it
-  __device__ __forceinline__ Stager(long long ld, int D, int lane, int wid) {
+  int wid, D;
+  __device__ __forceinline__ Stager(long long ld, int D_, int lane, int wid_) : wid(wid_), D(D_) {
     ldb = (uint32_t)ld * 2u;
     span = (uint32_t)(BK - 1) * ldb + (uint32_t)D * 2u;
-    row = wid * RP + lane / CH;
-    const int ch = (lane & (CH - 1)) ^ swz<DP>(row);
-    first = ch * 8 < D ? (uint32_t)row * ldb + (uint32_t)ch * 16u : 0x80000000u;
+    first = first_of(lane);
+  }
+  __device__ __forceinline__ uint32_t first_of(int lane) const {
+    const int row = wid * RP + lane / CH, ch = (lane & (CH - 1)) ^ swz<DP>(row);
+    return ch * 8 < D ? (uint32_t)row * ldb + (uint32_t)ch * 16u : 0x80000000u;
   }
   __device__ __forceinline__ rsrc_t tile(const uint16_t* src) const { return rsrc_of(src, span); }
-  // dst: the wave's first piece of the tile in LDS
-  __device__ __forceinline__ void piece(int i, rsrc_t rs, uint32_t dst, uint64_t rows) const {
-    uint32_t off = first;
-    if (rows != ~0ull) off = (rows >> (row + i * 4 * RP)) & 1 ? first : 0x80000000u;
-    dma16(rs, off, (uint32_t)(i * 4 * RP) * ldb, dst + i * 4096);
-  }
+  __device__ __forceinline__ uint32_t more(int i) const { return (uint32_t)(i * 4 * RP) * ldb; }  // piece i's offset behind the first's
+  // all pieces; dst: the wave's first piece of the tile in LDS
   __device__ __forceinline__ void all(const uint16_t* src, uint32_t dst, uint64_t rows) const {
     const rsrc_t rs = tile(src);
     rsrc_settled(rs);
+    if (rows == ~0ull) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) piece(i, rs, dst, rows);
+      for (int i = 0; i < PIECES; ++i) dma16(rs, first, more(i), dst + i * 4096);
+    } else {
+      const int row = wid * RP + fresh_lane() / CH;
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) dma16(rs, (rows >> (row + i * 4 * RP)) & 1 ? first : 0x80000000u, more(i), dst + i * 4096);
+    }
   }
 };
 // one row's operand fragments straight from memory (the operand that a wave keeps): zeros where `ok` is false and behind column D
@@ -146,11 +166,6 @@ __device__ __forceinline__ float max32(const f32x16 (&s)[2]) {
     for (int r = 1 + (u & 1) * 8; r + 1 < (u & 1 ? 16 : 9); r += 2) m[u] = max3(m[u], s[u >> 1][r], s[u >> 1][r + 1]);
   }
   return max3(max3(m[0], m[1], m[2]), m[3], max3(m[0], s[0][15], s[1][15]));
-}
-__device__ __forceinline__ float max16(const f32x16& s) {
-  const float first = fmaxf(s[0], s[1]);
-  const float a = max3(first, s[2], s[3]), b = max3(first, s[4], s[5]), c = max3(first, s[6], s[7]), d = max3(first, s[8], s[9]);
-  return max3(max3(a, s[10], s[11]), max3(b, s[12], s[13]), max3(max3(c, s[14], s[15]), d, d));
 }
 // the maximum with, and the sum with, the lane 32 further on, which holds the other half of the row
 struct Pair { float a, b; };
@@ -239,6 +254,25 @@ __device__ __forceinline__ uint64_t key_word(const int32_t* mask, int loaded, in
   return mask ? w & __ballot(loaded != 0) : w;
 }
 
+// LDS addresses of the fragments of a pair of tiles, in registers for the whole loop: what differs from use to use is an offset in the instruction
+template <int DP> struct Frags {
+  uint32_t rows[DP / 16], cols[DP / 16];  // of row fragments 0, 1, .. and of column fragments (dt, rows 0 / 8) of a tile
+  __device__ __forceinline__ Frags(uint32_t tile_rows, uint32_t tile_cols, int lane) {
+    const int g = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      rows[i] = tile_rows + tile_off<DP>(lane & 31, 2 * i + (lane >> 5));
+      const int col = (i >> 1) * 32 + ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2) + (i & 1) * 8;
+      cols[i] = tile_cols + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
+    }
+  }
+  template <int ROW> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))(rows[c] + ROW * DP * 2); }
+  template <int ROW> __device__ __forceinline__ bf16x8 col(int dt) const {
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt] + ROW * DP * 2)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt + 1] + ROW * DP * 2)));
+  }
+};
+
 // ------------------------------------------------------------------------------------------------ forward
 __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* lse, int tid) {
   const Gaps gap(a.seq_off, a.B, a.T);
@@ -252,7 +286,7 @@ __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* l
 // A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two
 // tiles each, so that a tile is on its way while the one before is worked on.
 template <int DP>
-__global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int fill) {
+__global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) fill_gaps(a, ctx, lse, tid);
@@ -264,78 +298,71 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
   const int last = min(tile.first + 127, n - 1), wlast = min(q0 + 31, n - 1);
   const int kbeg = max(tile.first - left, 0) & ~(BK - 1), kend = min(last + right + 1, n);
-  const uint16_t* kb_ = a.k + (long long)tile.row0 * a.k_row + kvh * a.k_head;
-  const uint16_t* vb_ = a.v + (long long)tile.row0 * a.v_row + kvh * a.v_head;
+  const int wbeg = max(q0 - left, 0), wend = q0 < n ? min(wlast + right + 1, n) : 0;  // the keys that this wave's rows see
+  const int allbeg = wlast - left, allend = q0 + right + 1;                           // ... that all of them see
+  const uint16_t* ks = a.k + (long long)(tile.row0 + kbeg) * a.k_row + kvh * a.k_head;  // the tile that is sent for next
+  const uint16_t* vs = a.v + (long long)(tile.row0 + kbeg) * a.v_row + kvh * a.v_head;
   const float sl2 = a.scale * kLog2e;
 
-  bf16x8 qf[DP / 16];
-  load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
-  landed(qf);
-  f32x16 o[DP / 32];
-#pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
-  float m = kLow, l = 0.f;
-
-  constexpr int TB = BK * DP * 2;  // bytes of a tile
-  const uint32_t lds0 = lds_addr(smem) + wid * 1024;  // (this wave's first piece)
+  constexpr int TB = BK * DP * 2, NC = DP / 16, ND = DP / 32;
+  const uint32_t mine = lds_addr(smem) + wid * 1024;  // (this wave's first piece)
   const Stager<DP> sk(a.k_row, a.dim, lane, wid), sv(a.v_row, a.dim, lane, wid);
   int loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
   uint64_t word = key_word(a.mask, loaded, n, kbeg);
   loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
-  if (kbeg < kend) {
-    sk.all(kb_ + kbeg * a.k_row, lds0, word);
-    sv.all(vb_ + kbeg * a.v_row, lds0 + TB, word);
-  }
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
-    const char* Kt = smem + buf * 2 * TB;
-    const char* Vt = Kt + TB;
+  sk.all(ks, mine, word);
+  sv.all(vs, mine + TB, word);
+
+  bf16x8 qf[NC];
+  load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
+  f32x16 o[ND];
+#pragma unroll
+  for (int dt = 0; dt < ND; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+  float m = kLow, l = 0.f;
+  const Frags<DP> f(lds_addr(smem), lds_addr(smem) + TB, lane);
+  landed(qf);
+
+  // one tile of keys from k0, in buffer BUF
+  auto work = [&](auto buf_, int k0) {
+    constexpr int BUF = decltype(buf_)::value, AT = BUF * 2 * BK;  // (the buffer's first row, in rows of DP)
     dma_wait();
     __syncthreads();
-    const uint64_t next = key_word(a.mask, loaded, n, k0 + BK);
+    const uint64_t now = word;
     if (k0 + BK < kend) {
-      const uint32_t to = lds0 + (buf ^ 1) * 2 * TB;
-      sk.all(kb_ + (long long)(k0 + BK) * a.k_row, to, next);
-      sv.all(vb_ + (long long)(k0 + BK) * a.v_row, to + TB, next);
+      word = key_word(a.mask, loaded, n, k0 + BK);
+      const uint32_t to = mine + (BUF ^ 1) * 2 * TB;
+      ks += BK * a.k_row;
+      vs += BK * a.v_row;
+      sk.all(ks, to, word);
+      sv.all(vs, to + TB, word);
       loaded = key_word_load(a.mask, tile.row0, n, k0 + 2 * BK, lane);
     }
-    const uint64_t now = word;
-    word = next;
-    if (q0 >= n || k0 > wlast + right || k0 + BK <= q0 - left || now == 0) continue;  // this wave's rows see nothing of the tile
+    if (k0 >= wend || k0 + BK <= wbeg) return;
     f32x16 s[2];
-    bf16x8 f0[DP / 16], f1[DP / 16];
+    bf16x8 f0[NC], f1[NC];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) f0[c] = frag_rows<DP>(Kt, 0, c, lane);
-    __builtin_amdgcn_sched_barrier(0);
+    for (int c = 0; c < NC; ++c) f0[c] = f.template row<AT>(c);
+    SCHED_FENCE();
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      f1[c] = frag_rows<DP>(Kt, 32, c, lane);
+    for (int c = 0; c < NC; ++c) {
+      f1[c] = f.template row<AT + 32>(c);
       s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0[c], qf[c], s[0], 0, 0, 0);
+      SCHED_FENCE();
     }
+    bf16x8 vf[ND];
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    for (int c = 0; c < NC; ++c) {
+      if (c % 2 == 0) vf[c / 2] = f.template col<AT>(c / 2);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1[c], qf[c], s[1], 0, 0, 0);
+      SCHED_FENCE();
     }
-    __builtin_amdgcn_sched_barrier(0);
-    bf16x8 vf[DP / 32];
-#pragma unroll
-    for (int dt = 0; dt < DP / 32; ++dt) vf[dt] = frag_cols<DP>(Vt, 0, dt, lane);
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1[c], qf[c], s[1], 0, 0, 0);
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    if (now != ~0ull || k0 < wlast - left || k0 + BK > q0 + right + 1) {
+    if (now != ~0ull || k0 < allbeg || k0 + BK > allend) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
         const int base = k0 + kb * 32;
@@ -350,13 +377,13 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
       m = up;
       l *= f;
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
+      for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] *= f;
     }
     // P of a 16-key step is made while the products of the step before run; the step's rows of V are fetched one step ahead
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    each<4>([&](auto t_) {
+      constexpr int t = decltype(t_)::value;
       float p[8];
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
@@ -365,348 +392,19 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
       }
       const bf16x8 pf = as_bf16x8(pack8(p));
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt) {
+      for (int dt = 0; dt < ND; ++dt) {
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], pf, o[dt], 0, 0, 0);
-        if (t < 3) vf[dt] = frag_cols<DP>(Vt, (t + 1) * 16, dt, lane);
+        if constexpr (t < 3) vf[dt] = f.template col<AT + (t + 1) * 16>(dt);
       }
-    }
+    });
+  };
+  for (int k0 = kbeg; k0 < kend; k0 += 2 * BK) {
+    work(std::integral_constant<int, 0>{}, k0);
+    if (k0 + BK < kend) work(std::integral_constant<int, 1>{}, k0 + BK);
   }
   l = sum_halves(l);
   if (qi < n && lane < 32) lse[(size_t)h * a.T + tile.row0 + qi] = l > 0.f ? (m + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
   store_T<DP>(ctx + (long long)(tile.row0 + qi) * a.o_row + h * a.o_head, o, l > 0.f || l != l ? 1.0f / l : 0.f, a.dim, qi < n, half);
-}
-
-// The same for long sequences, 64 query rows a wave and one wave a SIMD: every fragment of K and V that is read from LDS serves two products
-// instead of one.  With 32 rows a wave the fragments of a 128-wide head take 1128 clocks of the compute unit's LDS per tile, the products 1024 of the
-// matrix pipe.  With one wave there is no other to fill its waits, so the work is laid out for overlap in one instruction stream, in steps of 32 keys:
-//   the scores of step i (16 MFMAs)        beside   the first half of step i - 1's exponentials
-//   that half's 8 MFMAs of P V             beside   the second half's exponentials
-//   the second half's 8                    beside   the maximum of step i's scores
-// K and V have three tiles each, as the last step of a tile still reads V behind the barrier that opens the next.
-//
-// The 128 accumulators of the output stay in AGPRs: their products are asm statements (hipcc would copy accumulators to VGPRs and back around every
-// branch).  What reads or changes them comes behind s_nops (acc_scale, acc_done), as hipcc does not know that the matrix pipe wrote them.
-// FRESH: the B operand was packed just before (a vector instruction's result may be read by the matrix pipe two states later).
-template <bool FRESH> __device__ __forceinline__ void mfma_acc(f32x16& o, const bf16x8& x, const bf16x8& y) {
-  if constexpr (FRESH) asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(x), "v"(y));
-  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(o) : "v"(x), "v"(y));
-}
-#define ACC_MUL(i) "v_accvgpr_read_b32 %16, %" #i "\n\tv_mul_f32 %16, %16, %17\n\tv_accvgpr_write_b32 %" #i ", %16\n\t"
-__device__ __forceinline__ void acc_scale(f32x16& o, float f) {
-  float e[16], t;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) e[r] = o[r];
-  asm volatile("s_nop 15\n\ts_nop 15\n\t" ACC_MUL(0) ACC_MUL(1) ACC_MUL(2) ACC_MUL(3) ACC_MUL(4) ACC_MUL(5) ACC_MUL(6) ACC_MUL(7) ACC_MUL(8) ACC_MUL(9)
-                   ACC_MUL(10) ACC_MUL(11) ACC_MUL(12) ACC_MUL(13) ACC_MUL(14) ACC_MUL(15) "s_nop 4"
-               : "+a"(e[0]), "+a"(e[1]), "+a"(e[2]), "+a"(e[3]), "+a"(e[4]), "+a"(e[5]), "+a"(e[6]), "+a"(e[7]), "+a"(e[8]), "+a"(e[9]), "+a"(e[10]),
-                 "+a"(e[11]), "+a"(e[12]), "+a"(e[13]), "+a"(e[14]), "+a"(e[15]), "=&v"(t)
-               : "v"(f));
-#pragma unroll
-  for (int r = 0; r < 16; ++r) o[r] = e[r];
-}
-#undef ACC_MUL
-__device__ __forceinline__ void acc_done(f32x16& o) { asm volatile("s_nop 15\n\ts_nop 15" : "+a"(o)); }
-// scores: QA: that operand stays in AGPRs, too.  What reads the result comes behind other products or score_done
-template <bool FIRST, bool QA> __device__ __forceinline__ void mfma_score(f32x16& s, const bf16x8& k, const bf16x8& q) {
-  if constexpr (FIRST && QA) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "a"(q));
-  else if constexpr (FIRST) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s) : "v"(k), "v"(q));
-  else if constexpr (QA) asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "a"(q));
-  else asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s) : "v"(k), "v"(q));
-}
-__device__ __forceinline__ void score_done(f32x16 (&s)[2]) { asm volatile("s_nop 15\n\ts_nop 15" : "+v"(s[0]), "+v"(s[1])); }
-// f(0), f(1), .. f(N - 1) with the index as a constant
-template <int N, class F> __device__ __forceinline__ void each(F&& f) {
-  if constexpr (N > 0) {
-    each<N - 1>(f);
-    f(std::integral_constant<int, N - 1>{});
-  }
-}
-#define SCHED_FENCE() __builtin_amdgcn_sched_barrier(0)
-
-// A wave that is alone issues an instruction every 5 to 6 clocks, so their number counts as much as their kind: the LDS addresses of the fragments
-// live in registers and move by one addition a tile, and a tile whose rows are all there is sent for with three instructions a piece.
-template <int DP> struct Frags {
-  uint32_t rows[DP / 16], cols[DP / 16];  // of row fragments 0, 1, .. and of column fragments (dt, rows 0 / 8) of a tile
-  __device__ __forceinline__ Frags(uint32_t tile_rows, uint32_t tile_cols, int lane) {
-    const int g = lane >> 4, c = lane & 15;
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      rows[i] = tile_rows + tile_off<DP>(lane & 31, 2 * i + (lane >> 5));
-      const int col = (i >> 1) * 32 + ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2) + (i & 1) * 8;
-      cols[i] = tile_cols + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
-    }
-  }
-  static __device__ __forceinline__ void move(uint32_t (&at)[DP / 16], uint32_t by) {
-#pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      at[i] += by;
-      asm volatile("" : "+v"(at[i]));  // (it stays a register: hipcc would add it up again at every use)
-    }
-  }
-  template <int ROW> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))(rows[c] + ROW * DP * 2); }
-  template <int ROW> __device__ __forceinline__ bf16x8 col(int dt) const {
-    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt] + ROW * DP * 2)),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt + 1] + ROW * DP * 2)));
-  }
-};
-
-template <int DP>
-__global__ __launch_bounds__(256, 1) void attn_gqa_fwd2_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int fill) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  if (fill) fill_gaps(a, ctx, lse, tid);
-  const int slots = gridDim.x / a.heads, G = a.heads / a.kv_heads;
-  const int unit = blockIdx.x % a.heads, kvh = unit % a.kv_heads, h = kvh * G + unit / a.kv_heads;
-  const Tile tile = find_tile<256>(a.seq_off, a.B, a.T, slots - 1 - (int)(blockIdx.x / a.heads), lane);
-  if (tile.n == 0) return;
-  const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
-  const int q0 = tile.first + wid * 64, qi = q0 + (lane & 31);
-  const int last = min(tile.first + 255, n - 1), wlast = min(q0 + 63, n - 1);
-  const int kbeg = max(tile.first - left, 0) & ~(BK - 1), kend = min(last + right + 1, n);
-  const int wbeg = max(q0 - left, 0), wend = q0 < n ? min(wlast + right + 1, n) : 0;  // the keys that this wave's rows see
-  const int allbeg = wlast - left, allend = q0 + right + 1;                           // ... that all of them see
-  const uint16_t* ks = a.k + (long long)(tile.row0 + kbeg) * a.k_row + kvh * a.k_head;  // the tile that is sent for next
-  const uint16_t* vs = a.v + (long long)(tile.row0 + kbeg) * a.v_row + kvh * a.v_head;
-  const float sl2 = a.scale * kLog2e;
-
-  constexpr int TB = BK * DP * 2, PIECES = Stager<DP>::PIECES, NC = DP / 16, ND = DP / 32;
-  const uint32_t lds0 = lds_addr(smem), mine = lds0 + wid * 1024;  // (this wave's first piece)
-  const Stager<DP> sk(a.k_row, a.dim, lane, wid), sv(a.v_row, a.dim, lane, wid);
-  int loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
-  uint64_t word = key_word(a.mask, loaded, n, kbeg);
-  loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
-  sk.all(ks, mine, word);
-  sv.all(vs, mine + TB, word);
-
-  bf16x8 qf[2][NC];
-#pragma unroll
-  for (int b = 0; b < 2; ++b) load_frags<DP>(qf[b], a.q + (long long)(tile.row0 + qi + 32 * b) * a.q_row + h * a.q_head, a.dim, qi + 32 * b < n, half);
-  f32x16 o[2][ND];
-#pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[b][dt][r] = 0.f;
-  float m[2] = {kLow, kLow}, l[2] = {0.f, 0.f};
-  f32x16 sA[2], sB[2];  // the scores of a tile's first and second 32 keys
-#pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) sA[b][r] = sB[b][r] = -INFINITY;
-  Frags<DP> f(lds0, lds0 + TB, lane);
-  landed(qf[0]);
-  landed(qf[1]);
-#pragma unroll
-  for (int c = 0; c < NC; ++c) asm volatile("s_nop 1" : "+a"(qf[1][c]));  // (from here on in AGPRs)
-
-  // Registers 8 j + 2 i and the next of block b's scores: their exponentials, and from these the sum and the packed pair - a slot apart, as a
-  // result is 8 clocks away
-  float ex[2], ey[2];
-  auto expo = [&](const f32x16 (&s)[2], int r, int b, const float (&m)[2]) {
-    ex[b] = __builtin_amdgcn_exp2f(fmaf(s[b][r], sl2, -m[b]));
-    ey[b] = __builtin_amdgcn_exp2f(fmaf(s[b][r + 1], sl2, -m[b]));
-  };
-  auto pack = [&](uint32_t (&w)[2], int b) {
-    l[b] += ex[b];
-    w[b] = pack2bf(ex[b], ey[b]);
-    l[b] += ey[b];
-  };
-  auto operand = [](const uint32_t (&w)[4][2], int b) { return as_bf16x8(make_uint4(w[0][b], w[1][b], w[2][b], w[3][b])); };
-  // One step of 32 keys from k0 (rows ROW .. of the tile): its scores into s where the wave's rows see some of them (now), and the probabilities and
-  // products of the step before (scores sp, rows 32 - ROW .. of its tile; in front of a wave's first step an empty one, with scores of -inf).  send(i)
-  // sends for piece i of the next tile.
-  // Each product is followed by what fits into its 32 clocks.
-  auto step = [&](auto row_, int now, auto&& send, int k0, uint32_t word, f32x16 (&s)[2], const f32x16 (&sp)[2]) {
-    constexpr int ROW = decltype(row_)::value, RP = 32 - ROW;
-    bf16x8 vf[ND];
-    uint32_t w[4][2], x[4][2];
-    if (now) {
-      bf16x8 kf[NC];
-      SCHED_FENCE();
-#pragma unroll
-      for (int c = 0; c < NC / 2; ++c) kf[c] = f.template row<ROW>(c);
-      expo(sp, 0, 0, m);
-      expo(sp, 0, 1, m);
-      pack(w[0], 0);
-      pack(w[0], 1);
-      SCHED_FENCE();
-#pragma unroll
-      for (int t = 0; t < 2 * NC; ++t) {
-        const int c = t >> 1, b = t & 1;
-        if (t < 2) b ? mfma_score<true, true>(s[1], kf[0], qf[1][0]) : mfma_score<true, false>(s[0], kf[0], qf[0][0]);
-        else b ? mfma_score<false, true>(s[1], kf[c], qf[1][c]) : mfma_score<false, false>(s[0], kf[c], qf[0][c]);
-        if (b == 0) {
-          if (c + NC / 2 < NC) kf[c + NC / 2] = f.template row<ROW>(c + NC / 2);
-          else if (c - NC / 2 < ND) vf[c - NC / 2] = f.template col<RP>(c - NC / 2);
-        } else if (c % (NC / PIECES) == NC / PIECES - 1) send(c / (NC / PIECES));
-        // six pairs of registers are left: in every other slot of a half's exponentials, in the one behind it the sum
-        constexpr int PER = 2 * NC / 4;  // slots for one pair's two blocks
-        if (t / PER < 3) {
-          const int i = t / PER + 1, u = t % PER;
-          if (u == 0) expo(sp, 2 * i, 0, m);
-          if (u == PER / 4) pack(w[i], 0);
-          if (u == PER / 2) expo(sp, 2 * i, 1, m);
-          if (u == PER / 2 + PER / 4) pack(w[i], 1);
-        }
-        SCHED_FENCE();
-      }
-      if (word != ~0u || k0 < allbeg || k0 + 32 > allend) {
-        score_done(s);
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int at = qi + 32 * b - k0;
-          const uint32_t see = (bits32(at - left, at + right + 1) & word) >> (4 * half);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[b][r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[b][r] : -INFINITY;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) send(i);
-      float mm[2] = {m[0], m[1]};
-      asm volatile("" : "+v"(mm[0]), "+v"(mm[1]));  // (or hipcc makes the two branches' probabilities one, in front of both, beside nothing)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        expo(sp, 2 * i, 0, mm);
-        expo(sp, 2 * i, 1, mm);
-        pack(w[i], 0);
-        pack(w[i], 1);
-      }
-#pragma unroll
-      for (int dt = 0; dt < ND; ++dt) vf[dt] = f.template col<RP>(dt);
-    }
-    SCHED_FENCE();
-    float top[2];
-    {
-      bf16x8 vg[ND];
-      constexpr int UNITS = 8 / (2 * ND);  // (pair, block)s of the second half for each product of the first
-      each<2 * ND>([&](auto t_) {
-        constexpr int t = decltype(t_)::value, dt = t >> 1, b = t & 1;
-        mfma_acc<(t < 2)>(o[b][dt], vf[dt], operand(w, b));
-        if (b == 0) vg[dt] = f.template col<RP + 16>(dt);
-#pragma unroll
-        for (int u = t * UNITS; u < (t + 1) * UNITS; ++u) {
-          if (u > 0) pack(x[(u - 1) >> 1], (u - 1) & 1);
-          expo(sp, 8 + 2 * (u >> 1), u & 1, m);
-        }
-        SCHED_FENCE();
-      });
-      pack(x[3], 1);
-      float t0[2] = {0.f, 0.f}, t1[2] = {0.f, 0.f};
-      each<2 * ND>([&](auto t_) {
-        constexpr int t = decltype(t_)::value, dt = t >> 1, b = t & 1;
-        mfma_acc<(t < 2)>(o[b][dt], vg[dt], operand(x, b));
-        // the maximum of s[b] in two chains, four registers of each a slot
-#pragma unroll
-        for (int u = t * 8 / (2 * ND); u < (t + 1) * 8 / (2 * ND); ++u) {
-          const int y = u >> 1, q = u & 1;  // registers 4 y .. of block q
-          if (y == 0) t0[q] = t1[q] = fmaxf(s[q][0], s[q][1]);
-          t0[q] = max3(t0[q], s[q][4 * y], s[q][4 * y + 1]);
-          t1[q] = max3(t1[q], s[q][4 * y + 2], s[q][4 * y + 3]);
-        }
-        SCHED_FENCE();
-      });
-      top[0] = max3(t0[0], t1[0], t1[0]);
-      top[1] = max3(t0[1], t1[1], t1[1]);
-    }
-    if (now) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) top[b] = max_halves(top[b]) * sl2;
-      if (__any(top[0] > m[0] + kGrow || top[1] > m[1] + kGrow)) {
-        const bool old = __any((top[0] > m[0] + kGrow && m[0] > kLow) || (top[1] > m[1] + kGrow && m[1] > kLow));
-        float f[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const float up = top[b] > m[b] + kGrow ? top[b] : m[b];
-          f[b] = __builtin_amdgcn_exp2f(m[b] - up);
-          m[b] = up;
-          l[b] *= f[b];
-        }
-        if (old)  // (rows whose first maximum this is have their accumulators at zero, the others' factors are 1)
-          each<2 * ND>([&](auto i) { acc_scale(o[decltype(i)::value / ND][decltype(i)::value % ND], f[decltype(i)::value / ND]); });
-      }
-    }
-  };
-
-  // pieces of a whole tile: offsets of the wave's second, third, .. from its first
-  uint32_t ko[PIECES], vo[PIECES];
-#pragma unroll
-  for (int i = 0; i < PIECES; ++i) {
-    ko[i] = (uint32_t)(i * 4 * Stager<DP>::RP) * sk.ldb;
-    vo[i] = (uint32_t)(i * 4 * Stager<DP>::RP) * sv.ldb;
-  }
-  int buf = 0;
-  int open = 0;
-  uint32_t shift = 0;  // from the tile before to this one
-  for (int k0 = kbeg; k0 < kend; k0 += BK) {
-    dma_wait();
-    __syncthreads();
-    const uint64_t now = word;
-    word = key_word(a.mask, loaded, n, k0 + BK);
-    const int ahead = buf == 2 ? 0 : buf + 1;
-    const uint32_t to = mine + ahead * 2 * TB;
-    ks += BK * a.k_row;
-    vs += BK * a.v_row;
-    const rsrc_t rk = sk.tile(ks), rv = sv.tile(vs);
-    // The next tile's K is sent for during the first step, its V during the second (eight pieces at once would hold the wave for over 1000 clocks) -
-    // if all its rows are there: else at once.
-    const int whole = __builtin_amdgcn_readfirstlane(k0 + BK < kend && word == ~0ull);
-    if (k0 + BK < kend) {
-      loaded = key_word_load(a.mask, tile.row0, n, k0 + 2 * BK, lane);
-      rsrc_settled(rk);
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) {
-          sk.piece(i, rk, to, word);
-          sv.piece(i, rv, to + TB, word);
-        }
-      }
-    }
-    auto send_k = [&](int i) { if (whole) dma16(rk, sk.first, ko[i], to + i * 4096); };
-    auto send_v = [&](int i) { if (whole) dma16(rv, sv.first, vo[i], to + TB + i * 4096); };
-    const int first = __builtin_amdgcn_readfirstlane(k0 < wend && k0 + 32 > wbeg), second = __builtin_amdgcn_readfirstlane(k0 + 32 < wend && k0 + 64 > wbeg);
-    Frags<DP>::move(f.rows, shift);
-    if (first || open) step(std::integral_constant<int, 0>{}, first, send_k, k0, (uint32_t)now, sA, sB);
-    else {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) send_k(i);
-    }
-    Frags<DP>::move(f.cols, shift);
-    if (second || first) step(std::integral_constant<int, 32>{}, second, send_v, k0 + 32, (uint32_t)(now >> 32), sB, sA);
-    else {
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) send_v(i);
-    }
-    open = second;
-    shift = ahead == 0 ? -4 * TB : 2 * TB;
-    buf = ahead;
-  }
-  if (open) {  // the last step's probabilities and products
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      uint32_t w[4][2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          expo(sB, j * 8 + 2 * i, b, m);
-          pack(w[i], b);
-        }
-      each<2 * ND>([&](auto t_) {
-        constexpr int t = decltype(t_)::value, dt = t >> 1, b = t & 1;
-        mfma_acc<true>(o[b][dt], j == 0 ? f.template col<32>(dt) : f.template col<48>(dt), operand(w, b));
-      });
-    }
-  }
-  each<2 * ND>([&](auto i) { acc_done(o[decltype(i)::value / ND][decltype(i)::value % ND]); });
-#pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int row = qi + 32 * b;
-    const float t = sum_halves(l[b]);
-    if (row < n && lane < 32) lse[(size_t)h * a.T + tile.row0 + row] = t > 0.f ? (m[b] + __log2f(t)) * kLn2 : (t == 0.f ? -INFINITY : t);
-    store_T<DP>(ctx + (long long)(tile.row0 + row) * a.o_row + h * a.o_head, o[b], t > 0.f || t != t ? 1.0f / t : 0.f, a.dim, row < n, half);
-  }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -739,7 +437,8 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
   load_frags<DP>(df, dctx + (long long)(tile.row0 + qi) * a.do_row + h * a.do_head, a.dim, qi < n, half);
   const size_t at = (size_t)h * a.T + tile.row0 + qi;
-  float nl = qi < n ? -lse[at] * kLog2e : 0.f;
+  // (an empty row's lse is -inf: its probabilities are exp2(s - inf) = 0, whatever s is)
+  float nl = qi < n ? (lse[at] == -INFINITY ? -INFINITY : -lse[at] * kLog2e) : 0.f;
   asm volatile("s_waitcnt vmcnt(0)" : "+v"(nl));
   float nd = 0.f;
   {
@@ -825,9 +524,29 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   store_T<DP>(dq + (long long)(tile.row0 + qi) * a.dq_row + h * a.dq_head, acc, a.scale, a.dim, qi < n, half);
 }
 
-// dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows
+// LDS address of a fragment as the address of fragment 0 with a few bits flipped: a tile's rows start at multiples of DP * 2 bytes, so the chunk
+// number and its permutation are address bits of their own, and one register and an exclusive or do for eight.
+template <int DP> struct Bits {
+  uint32_t rows, cols;
+  __device__ __forceinline__ Bits(uint32_t at, int lane) {
+    const int g = lane >> 4, c = lane & 15, col = ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2);
+    rows = at + tile_off<DP>(lane & 31, lane >> 5);
+    cols = at + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
+  }
+  // what they are is forgotten: or hipcc makes the flipped addresses once, in front of the loop, and keeps each in a register of its own
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(rows), "+v"(cols)); }
+  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))((rows ^ (c << 5)) + AT); }
+  // rows + 8 flip bit 1 of the permutation (DP = 128: row bit 3 is its bit 1; DP = 64: row bit 3 its bit 1, too)
+  template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ (dt << 6)) + AT)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ ((dt << 6) | 32)) + AT + 8 * DP * 2)));
+  }
+};
+
+// dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows.  The wave's
+// K and V fragments and its 128 accumulators stay in registers: 256 of them are just enough, and leave room for a second wave on the SIMD.
 template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
+__global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
                                                               int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -850,90 +569,150 @@ __global__ __launch_bounds__(256, DP == 64 ? 2 : 1) void attn_gqa_dkv_kernel(con
   const int qbeg = max(tile.first - right, 0) & ~(BK - 1), qend = min(last + left + 1, n);
   const float sl2 = a.scale * kLog2e;
   const bool alive = kj < n && (!a.mask || a.mask[tile.row0 + kj] != 0);
-  const bool all = __all(alive), none = !__any(alive);
+  const uint32_t live = (uint32_t)__ballot(alive);  // (both halves of the wave have the same 32 keys)
 
-  bf16x8 kf[DP / 16], vf[DP / 16];
+  constexpr int TB = BK * DP * 2, SB = 2 * TB + 2 * BK * 4, NC = DP / 16, ND = DP / 32;  // Q tile, dO tile, -lse and -delta of the rows
+  const int tiles = qend > qbeg ? (qend - qbeg + BK - 1) / BK : 0, steps = tiles * G;
+  const uint32_t lds0 = lds_addr(smem);
+  Stager<DP> sq(a.q_row, a.dim, lane, wid), sd(a.do_row, a.dim, lane, wid);
+  // the tile that is sent for next: its first row, where its Q, dO and statistics are, and from there to the next head's first tile
+  int fq = qbeg;
+  const uint16_t* qs = a.q + (long long)(tile.row0 + qbeg) * a.q_row + kvh * G * a.q_head;
+  const uint16_t* ds = dctx + (long long)(tile.row0 + qbeg) * a.do_row + kvh * G * a.do_head;
+  const float* st = (wid == 0 ? nlse : ndelta) + (size_t)kvh * G * a.T + tile.row0 + qbeg;
+  auto fetch = [&](uint32_t to) {
+    const uint64_t rows = bits_below(n - fq);
+    const int l = fresh_lane();
+    sq.first = sq.first_of(l);
+    sd.first = sd.first_of(l);
+    sq.all(qs, to + wid * 1024, rows);
+    sd.all(ds, to + TB + wid * 1024, rows);
+    if (wid < 2) {
+      const rsrc_t rs = rsrc_of(st, (uint32_t)min(n - fq, BK) * 4u);
+      rsrc_settled(rs);
+      dma4(rs, (uint32_t)fresh_lane() * 4u, to + 2 * TB + wid * BK * 4);
+    }
+    fq += BK;
+    qs += BK * a.q_row;
+    ds += BK * a.do_row;
+    st += BK;
+    if (fq >= qend) {
+      const int back = fq - qbeg;
+      fq = qbeg;
+      qs += a.q_head - back * a.q_row;
+      ds += a.do_head - back * a.do_row;
+      st += a.T - back;
+    }
+  };
+  if (steps) fetch(lds0);
+
+  bf16x8 kf[NC], vf[NC];
   load_frags<DP>(kf, a.k + (long long)(tile.row0 + kj) * a.k_row + kvh * a.k_head, a.dim, alive, half);
   load_frags<DP>(vf, a.v + (long long)(tile.row0 + kj) * a.v_row + kvh * a.v_head, a.dim, alive, half);
   landed(kf);
   landed(vf);
-  f32x16 gk[DP / 32], gv[DP / 32];
+  // (of the 128-wide head's fragments one is kept in LDS, each lane its own, and read when it is needed: in registers it is the one too many)
+  constexpr bool LENT = DP == 128;
+  if constexpr (LENT) *(LDS_PTR(bf16x8))(lds0 + 2 * SB + tid * 16) = kf[NC - 1];
+  f32x16 gk[ND], gv[ND];
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt)
+  for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) { gk[dt][r] = 0.f; gv[dt][r] = 0.f; }
+  Bits<DP> f(lds0, lane);
 
-  constexpr int TB = BK * DP * 2, SB = 2 * TB + 2 * BK * 4;  // Q tile, dO tile, -lse and -delta of the rows
-  const int tiles = qend > qbeg ? (qend - qbeg + BK - 1) / BK : 0, steps = tiles * G;
-  const uint32_t lds0 = lds_addr(smem);
-  const Stager<DP> sq(a.q_row, a.dim, lane, wid), sd(a.do_row, a.dim, lane, wid);
-  auto fetch = [&](int i, uint32_t to) {
-    const int h = kvh * G + i / tiles, q0 = qbeg + (i % tiles) * BK;
-    const uint64_t rows = bits_below(n - q0);
-    sq.all(a.q + (long long)(tile.row0 + q0) * a.q_row + h * a.q_head, to + wid * 1024, rows);
-    sd.all(dctx + (long long)(tile.row0 + q0) * a.do_row + h * a.do_head, to + TB + wid * 1024, rows);
-    if (wid < 2) {
-      const rsrc_t rs = rsrc_of((wid == 0 ? nlse : ndelta) + (size_t)h * a.T + tile.row0 + q0, (uint32_t)min(n - q0, BK) * 4u);
-      rsrc_settled(rs);
-      dma4(rs, (uint32_t)lane * 4u, to + 2 * TB + wid * BK * 4);
-    }
-  };
-  if (steps) fetch(0, lds0);
-  for (int i = 0; i < steps; ++i) {
-    const char* Qt = smem + (i & 1) * SB;
-    const char* Dt = Qt + TB;
-    const float* nl = reinterpret_cast<const float*>(Qt + 2 * TB);
-    const float* nd = nl + BK;
+  int q0 = qbeg, left_ = steps;  // the tile that is worked on, the tiles that are left
+  auto work = [&](auto buf_) {
+    constexpr int QA = decltype(buf_)::value * SB, DA = QA + TB;
     dma_wait();
     __syncthreads();
-    if (i + 1 < steps) fetch(i + 1, lds0 + ((i + 1) & 1) * SB);
-    const int q0 = qbeg + (i % tiles) * BK;
-    if (none || q0 > wlast + left || q0 + BK <= key0 - right) continue;
-    const bool edge = !all || q0 < wlast - right || q0 + BK > key0 + left + 1;
-#pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
+    if (--left_ > 0) fetch(lds0 + (decltype(buf_)::value ^ 1) * SB);
+    const int at = q0;
+    q0 = q0 + BK >= qend ? qbeg : q0 + BK;
+    if (live == 0 || at > wlast + left || at + BK <= key0 - right) return;
+    const bool edge = live != ~0u || at < wlast - right || at + BK > key0 + left + 1;
+    each<2>([&](auto qb_) {
+      constexpr int qb = decltype(qb_)::value, Q = QA + qb * 32 * DP * 2, D = DA + qb * 32 * DP * 2;
+      // (fragments are read DEEP - 1 ahead of their products: more do not fit)
+      constexpr int DEEP = 2;
+      f.forget();
+      const uint32_t stat = lds0 + 2 * TB + 16 * (fresh_lane() >> 5);
       f32x16 s, dp;
+      bf16x8 x[DEEP], kl;
+      SCHED_FENCE();
 #pragma unroll
-      for (int rg = 0; rg < 4; ++rg) {
-        const float4 d4 = *reinterpret_cast<const float4*>(nd + qb * 32 + 8 * rg + 4 * half);
-        dp[rg * 4] = d4.x; dp[rg * 4 + 1] = d4.y; dp[rg * 4 + 2] = d4.z; dp[rg * 4 + 3] = d4.w;
-        s[rg * 4] = s[rg * 4 + 1] = s[rg * 4 + 2] = s[rg * 4 + 3] = 0.f;
+      for (int c = 0; c < DEEP - 1; ++c) x[c] = f.template row<Q>(c);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        SCHED_FENCE();
+        const int u = c + DEEP - 1;
+        x[u % DEEP] = u < NC ? f.template row<Q>(u) : f.template row<D>(u - NC);
+        if (LENT && c == NC - 2) kl = *(const LDS_PTR(bf16x8))(lds0 + 2 * SB + wid * 1024 + fresh_lane() * 16);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % DEEP], LENT && c == NC - 1 ? kl : kf[c], s, 0, 0, 0);
       }
-#pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows<DP>(Qt, qb * 32, c, lane), kf[c], s, 0, 0, 0);
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows<DP>(Dt, qb * 32, c, lane), vf[c], dp, 0, 0, 0);
-      }
-      float p[16], ds[16];
-#pragma unroll
-      for (int rg = 0; rg < 4; ++rg) {
-        const float4 l4 = *reinterpret_cast<const float4*>(nl + qb * 32 + 8 * rg + 4 * half);
-        const float ll[4] = {l4.x, l4.y, l4.z, l4.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[rg * 4 + e] = __builtin_amdgcn_exp2f(fmaf(s[rg * 4 + e], sl2, ll[e]));
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = p[r] * dp[r];
+      SCHED_FENCE();
       if (edge) {
-        const int base = q0 + qb * 32;
-        const uint32_t see = alive ? bits32(kj - right - base, min(kj + left + 1, n) - base) >> (4 * half) : 0u;
+        const int l = fresh_lane(), key = key0 + (l & 31), base = at + qb * 32;
+        const uint32_t see = (live >> (l & 31)) & 1 ? bits32(key - right - base, min(key + left + 1, n) - base) >> (4 * (l >> 5)) : 0u;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const bool is = (see >> (8 * (r >> 2) + (r & 3))) & 1;
-          p[r] = is ? p[r] : 0.f;
-          ds[r] = is ? ds[r] : 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+      }
+      SCHED_FENCE();
+#pragma unroll
+      for (int rg = 0; rg < 4; ++rg) {  // dP starts at -delta of its rows
+        const f32x4 d4 = *(const LDS_PTR(f32x4))(stat + decltype(buf_)::value * SB + BK * 4 + qb * 128 + 32 * rg);
+        dp[rg * 4] = d4[0]; dp[rg * 4 + 1] = d4[1]; dp[rg * 4 + 2] = d4[2]; dp[rg * 4 + 3] = d4[3];
+      }
+      // beside the products of dP: the probabilities, two registers a product
+      f32x4 l4;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        SCHED_FENCE();
+        const int u = c + DEEP - 1;
+        if (u < NC) x[(NC + u) % DEEP] = f.template row<D>(u);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[(NC + c) % DEEP], vf[c], dp, 0, 0, 0);
+#pragma unroll
+        for (int e = c * 16 / NC; e < (c + 1) * 16 / NC; ++e) {
+          if (e % 4 == 0) l4 = *(const LDS_PTR(f32x4))(stat + decltype(buf_)::value * SB + qb * 128 + 8 * e);
+          s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sl2, l4[e % 4]));
         }
       }
+      SCHED_FENCE();
+      bf16x8 pf[2], df[2], z[DEEP];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const bf16x8 pf = pack_acc(p, j), sf = pack_acc(ds, j);
+        float p[8], d[8];
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt) {
-          gv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols<DP>(Dt, qb * 32 + j * 16, dt, lane), pf, gv[dt], 0, 0, 0);
-          gk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols<DP>(Qt, qb * 32 + j * 16, dt, lane), sf, gk[dt], 0, 0, 0);
+        for (int e = 0; e < 8; ++e) {
+          p[e] = s[j * 8 + e];
+          d[e] = s[j * 8 + e] * dp[j * 8 + e];
         }
+        pf[j] = as_bf16x8(pack8(p));
+        df[j] = as_bf16x8(pack8(d));
+        SCHED_FENCE();
       }
-    }
+      // the steps j of 16 rows: dV's products, then dK's.  fragment k = 2 ND j + ND (dK) + dt
+      auto frag = [&](auto k_) {
+        constexpr int k = decltype(k_)::value, j = k / (2 * ND), dt = k % ND;
+        if constexpr (k % (2 * ND) < ND) return f.template col<D + j * 16 * DP * 2>(dt);
+        else return f.template col<Q + j * 16 * DP * 2>(dt);
+      };
+      each<DEEP - 1>([&](auto k) { z[decltype(k)::value] = frag(k); });
+      each<4 * ND>([&](auto k_) {
+        constexpr int k = decltype(k_)::value, j = k / (2 * ND), dt = k % ND, u = k + DEEP - 1;
+        SCHED_FENCE();
+        if constexpr (u < 4 * ND) z[u % DEEP] = frag(std::integral_constant<int, u>{});
+        if constexpr (k % (2 * ND) < ND) gv[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(z[k % DEEP], pf[j], gv[dt], 0, 0, 0);
+        else gk[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(z[k % DEEP], df[j], gk[dt], 0, 0, 0);
+      });
+      SCHED_FENCE();
+    });
+  };
+  while (left_ > 0) {
+    work(std::integral_constant<int, 0>{});
+    if (left_ > 0) work(std::integral_constant<int, 1>{});
   }
   const long long row = tile.row0 + kj;
   store_T<DP>(dk + row * a.dk_row + kvh * a.dk_head, gk, a.scale, a.dim, kj < n, half);
@@ -967,15 +746,12 @@ int check(const Args* a, const char* what) {
   return COCODR_OK;
 }
 
-bool long_rows(const Args* a) { return a->T / a->B >= 512; }
 template <class K> void allow_lds(K kernel, int bytes) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 constexpr int kv_lds(int DP) { return 4 * BK * DP * 2; }
-constexpr int kv3_lds(int DP) { return 6 * BK * DP * 2; }
-constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4); }
+constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4) + (DP == 128 ? 4096 : 0); }
 void lds_limits() {
   static cocodr_lds_once once;
   if (!once.pending()) return;
-  allow_lds(attn_gqa_fwd2_kernel<64>, kv3_lds(64)); allow_lds(attn_gqa_fwd2_kernel<128>, kv3_lds(128));
   allow_lds(attn_gqa_fwd_kernel<64>, kv_lds(64)); allow_lds(attn_gqa_fwd_kernel<128>, kv_lds(128));
   allow_lds(attn_gqa_dq_kernel<64>, kv_lds(64)); allow_lds(attn_gqa_dq_kernel<128>, kv_lds(128));
   allow_lds(attn_gqa_dkv_kernel<64>, qd_lds(64)); allow_lds(attn_gqa_dkv_kernel<128>, qd_lds(128));
@@ -991,11 +767,7 @@ extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* a, uint16_t* ctx,
   lds_limits();
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)((a->T / 128 + a->B) * a->heads));
-  if (long_rows(a)) {
-    const dim3 grid2((unsigned)((a->T / 256 + a->B) * a->heads));
-    if (a->dim <= 64) hipLaunchKernelGGL(attn_gqa_fwd2_kernel<64>, grid2, dim3(256), kv3_lds(64), st, *a, ctx, lse, fill);
-    else hipLaunchKernelGGL(attn_gqa_fwd2_kernel<128>, grid2, dim3(256), kv3_lds(128), st, *a, ctx, lse, fill);
-  } else if (a->dim <= 64) hipLaunchKernelGGL(attn_gqa_fwd_kernel<64>, grid, dim3(256), kv_lds(64), st, *a, ctx, lse, fill);
+  if (a->dim <= 64) hipLaunchKernelGGL(attn_gqa_fwd_kernel<64>, grid, dim3(256), kv_lds(64), st, *a, ctx, lse, fill);
   else hipLaunchKernelGGL(attn_gqa_fwd_kernel<128>, grid, dim3(256), kv_lds(128), st, *a, ctx, lse, fill);
   CK_LAUNCH("attn_gqa_fwd");
   return COCODR_OK;
