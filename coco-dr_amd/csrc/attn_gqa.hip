@@ -204,22 +204,68 @@ template <int DP> __device__ __forceinline__ void store_T(uint16_t* row, const f
 struct Tile {
   int n, first, row0;  // the sequence's rows (0: nothing to do), this tile's first row in it, the sequence's first row in the buffer
 };
-template <int TILE> __device__ __forceinline__ Tile find_tile(const int32_t* off, int B, int T, int num, int lane) {
-  int lo = 0, n = B;
-  while (n > 1) {
-    const int step = (n + 63) >> 6;
-    const int at = lo + lane * step;
-    bool below = false;
-    if (lane * step < n) below = min(max(off[at], 0), T) / TILE + at <= num;
-    const int c = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(below)));
-    if (c == 0) break;
-    const int cut = (c - 1) * step;
-    n = min(step, n - cut);
-    lo += cut;
+//
+// When sequences are long and few (by_work), the numbers go by the work of a tile instead, the most first: a workgroup with much to do that starts
+// among the last is waited for by an empty chip.  A lane then has a sequence of c tiles.
+//   kUp, kDown: the work grows (falls) along a sequence, so tile x (tile c - 1 - x) of every sequence that has it comes before tile x - 1:
+//     x is the largest with S(x) = sum max(c - x, 0) > number, found 64 candidates at a time
+//   kLevel: it is the same along a sequence: all tiles of the longest sequence, then of the next
+enum Order { kPlain, kUp, kDown, kLevel };
+__device__ __forceinline__ int tiles_from(int c, int B, int x) {  // S(x); x may differ from lane to lane
+  int sum = 0;
+  for (int b = 0; b < B; ++b) sum += max(__builtin_amdgcn_readlane(c, b) - x, 0);
+  return sum;
+}
+template <int TILE> __device__ __forceinline__ Tile find_tile(const int32_t* off, int B, int T, int num, int order, int lane) {
+  int lo = 0, n = B, t = -1;
+  if (order == kPlain) {
+    while (n > 1) {
+      const int step = (n + 63) >> 6;
+      const int at = lo + lane * step;
+      bool below = false;
+      if (lane * step < n) below = min(max(off[at], 0), T) / TILE + at <= num;
+      const int c = __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(below)));
+      if (c == 0) break;
+      const int cut = (c - 1) * step;
+      n = min(step, n - cut);
+      lo += cut;
+    }
+  } else {
+    int c = 0;
+    if (lane < B) {
+      const int a = min(max(off[lane], 0), T);
+      c = (min(max(off[lane + 1], a), T) - a + TILE - 1) / TILE;
+    }
+    bool here;
+    if (order == kLevel) {
+      int start = 0;
+      for (int b = 0; b < B; ++b) {
+        const int other = __builtin_amdgcn_readlane(c, b);
+        start += other > c || (other == c && b < lane) ? other : 0;
+      }
+      t = num - start;
+      here = t >= 0 && t < c;
+    } else {
+      int x = 0, span = T / TILE + 1;
+      while (span > 1) {
+        const int step = (span + 63) >> 6;
+        const bool more = lane * step < span && tiles_from(c, B, x + lane * step) > num;
+        const int cut = max(__builtin_amdgcn_readfirstlane((int)__popcll(__ballot(more))) - 1, 0) * step;
+        span = min(step, span - cut);
+        x += cut;
+      }
+      const uint64_t have = __ballot(c > x);
+      here = c > x && (int)__popcll(have & ((1ull << lane) - 1)) == num - tiles_from(c, B, x + 1);
+      t = order == kUp ? x : c - 1 - x;
+    }
+    const uint64_t found = __ballot(here);
+    if (found == 0) return Tile{0, 0, 0};
+    lo = __ffsll((long long)found) - 1;
+    t = __builtin_amdgcn_readlane(t, __builtin_amdgcn_readfirstlane(lo));
   }
   lo = __builtin_amdgcn_readfirstlane(lo);
   const int a = min(max(off[lo], 0), T), e = min(max(off[lo + 1], a), T);
-  const int t = num - (a / TILE + lo);
+  if (order == kPlain) t = num - (a / TILE + lo);
   Tile r;
   r.n = t >= 0 && t < (e - a + TILE - 1) / TILE ? e - a : 0;
   r.first = t * TILE;
@@ -286,13 +332,13 @@ __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* l
 // A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two
 // tiles each, so that a tile is on its way while the one before is worked on.
 template <int DP>
-__global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int fill) {
+__global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) fill_gaps(a, ctx, lse, tid);
   const int slots = gridDim.x / a.heads, G = a.heads / a.kv_heads;
   const int unit = blockIdx.x % a.heads, kvh = unit % a.kv_heads, h = kvh * G + unit / a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, slots - 1 - (int)(blockIdx.x / a.heads), lane);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, order == kPlain ? slots - 1 - (int)(blockIdx.x / a.heads) : (int)(blockIdx.x / a.heads), order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
@@ -413,7 +459,7 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(con
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,
                                                              const float* __restrict__ lse, float* __restrict__ ndelta, float* __restrict__ nlse,
-                                                             uint16_t* __restrict__ dq, int fill) {
+                                                             uint16_t* __restrict__ dq, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) {
@@ -423,7 +469,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   }
   const int slots = gridDim.x / a.heads, G = a.heads / a.kv_heads;
   const int unit = blockIdx.x % a.heads, kvh = unit % a.kv_heads, h = kvh * G + unit / a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, slots - 1 - (int)(blockIdx.x / a.heads), lane);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, order == kPlain ? slots - 1 - (int)(blockIdx.x / a.heads) : (int)(blockIdx.x / a.heads), order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
@@ -548,7 +594,7 @@ template <int DP> struct Bits {
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                                                              int fill) {
+                                                              int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) {
@@ -561,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
       }
   }
   const int G = a.heads / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, blockIdx.x / a.kv_heads, lane);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, blockIdx.x / a.kv_heads, order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int key0 = tile.first + wid * 32, kj = key0 + (lane & 31);
@@ -746,6 +792,14 @@ int check(const Args* a, const char* what) {
   return COCODR_OK;
 }
 
+// by work: where tiles have so much of it (sequences of 256 rows and more on average) that the longer search for them does not count, where their work
+// differs (no window on both sides), and where a lane each does for the sequences
+Order order_of(const Args* a, bool keys) {
+  if (a->B > 64 || a->T / a->B < 256 || (a->left >= 0 && a->right >= 0)) return kPlain;
+  if (a->left < 0 && a->right < 0) return kLevel;
+  return (a->right >= 0) != keys ? kUp : kDown;
+}
+
 template <class K> void allow_lds(K kernel, int bytes) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 constexpr int kv_lds(int DP) { return 4 * BK * DP * 2; }
 constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4) + (DP == 128 ? 4096 : 0); }
@@ -767,8 +821,8 @@ extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* a, uint16_t* ctx,
   lds_limits();
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)((a->T / 128 + a->B) * a->heads));
-  if (a->dim <= 64) hipLaunchKernelGGL(attn_gqa_fwd_kernel<64>, grid, dim3(256), kv_lds(64), st, *a, ctx, lse, fill);
-  else hipLaunchKernelGGL(attn_gqa_fwd_kernel<128>, grid, dim3(256), kv_lds(128), st, *a, ctx, lse, fill);
+  if (a->dim <= 64) hipLaunchKernelGGL(attn_gqa_fwd_kernel<64>, grid, dim3(256), kv_lds(64), st, *a, ctx, lse, order_of(a, false), fill);
+  else hipLaunchKernelGGL(attn_gqa_fwd_kernel<128>, grid, dim3(256), kv_lds(128), st, *a, ctx, lse, order_of(a, false), fill);
   CK_LAUNCH("attn_gqa_fwd");
   return COCODR_OK;
 }
@@ -793,11 +847,11 @@ extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t
   float *ndelta = workspace, *nlse = workspace + (size_t)a->T * a->heads;
   const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)((a->T / 128 + a->B) * a->kv_heads));
   if (a->dim <= 64) {
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, fill);
-    hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, fill);
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, order_of(a, false), fill);
+    hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, order_of(a, true), fill);
   } else {
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, fill);
-    hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, fill);
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, order_of(a, false), fill);
+    hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, order_of(a, true), fill);
   }
   CK_LAUNCH("attn_gqa_bwd");
   return COCODR_OK;
