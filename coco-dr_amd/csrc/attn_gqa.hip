@@ -589,12 +589,23 @@ template <int DP> struct Bits {
   }
 };
 
+// the tiles of queries that see a tile of 128 keys, and in how many parts a group's heads are summed for it
+__device__ __forceinline__ int query_tiles(const Args& a, const Tile& t) {
+  const int beg = max(t.first - (a.right < 0 ? kFar : a.right), 0) & ~(BK - 1);
+  const int end = min(min(t.first + 127, t.n - 1) + (a.left < 0 ? kFar : a.left) + 1, t.n);
+  return end > beg ? (end - beg + BK - 1) / BK : 0;
+}
+// A part's sums are 2 x 128 x D fp32 written and read again: 262 KB at D = 128, about as long as 4 steps of 64 queries.  Tiles of up to kWhole steps are left whole:
+// 16 sequences of 1 to 2048 (log), 32 / 8 heads of 128, causal, forward and backward: 505 / 496 / 579 us with 16 / 48 / 96.
+constexpr int kWhole = 48;
+__device__ __forceinline__ int split_of(int steps, int split) { return steps > kWhole ? split : 1; }
+
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows.  The wave's
 // K and V fragments and its 128 accumulators stay in registers: 256 of them are just enough, and leave room for a second wave on the SIMD.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                                                              int order, int fill) {
+                                                              f32x4* __restrict__ part, int split, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) {
@@ -606,26 +617,31 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
         *reinterpret_cast<uint2*>(dv + row * a.dv_row + h * a.dv_head + tid * 4) = make_uint2(0u, 0u);
       }
   }
-  const int G = a.heads / a.kv_heads, kvh = blockIdx.x % a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, blockIdx.x / a.kv_heads, order, lane);
+  const int kvh = blockIdx.x % a.kv_heads, sub = blockIdx.x / a.kv_heads % split, num = blockIdx.x / (a.kv_heads * split);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, num, order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int key0 = tile.first + wid * 32, kj = key0 + (lane & 31);
   const int last = min(tile.first + 127, n - 1), wlast = min(key0 + 31, n - 1);
   const int qbeg = max(tile.first - right, 0) & ~(BK - 1), qend = min(last + left + 1, n);
+  const int tiles = query_tiles(a, tile), heads = a.heads / a.kv_heads, G = heads / split_of(tiles * heads, split);  // (heads that this workgroup has)
+  if (sub * G >= heads) return;
+  f32x4* to = G < heads ? part + ((size_t)(num * a.kv_heads + kvh) * split + sub) * (DP / 4 * 256) : nullptr;  // where this part's sums go
   const float sl2 = a.scale * kLog2e;
   const bool alive = kj < n && (!a.mask || a.mask[tile.row0 + kj] != 0);
   const uint32_t live = (uint32_t)__ballot(alive);  // (both halves of the wave have the same 32 keys)
 
   constexpr int TB = BK * DP * 2, SB = 2 * TB + 2 * BK * 4, NC = DP / 16, ND = DP / 32;  // Q tile, dO tile, -lse and -delta of the rows
-  const int tiles = qend > qbeg ? (qend - qbeg + BK - 1) / BK : 0, steps = tiles * G;
+  const int steps = tiles * G, h0 = kvh * heads + sub * G;
   const uint32_t lds0 = lds_addr(smem);
   Stager<DP> sq(a.q_row, a.dim, lane, wid), sd(a.do_row, a.dim, lane, wid);
   // the tile that is sent for next: its first row, where its Q, dO and statistics are, and from there to the next head's first tile
   int fq = qbeg;
-  const uint16_t* qs = a.q + (long long)(tile.row0 + qbeg) * a.q_row + kvh * G * a.q_head;
-  const uint16_t* ds = dctx + (long long)(tile.row0 + qbeg) * a.do_row + kvh * G * a.do_head;
-  const float* st = (wid == 0 ? nlse : ndelta) + (size_t)kvh * G * a.T + tile.row0 + qbeg;
+  const uint16_t* qs = a.q + (long long)(tile.row0 + qbeg) * a.q_row + h0 * a.q_head;
+  const uint16_t* ds = dctx + (long long)(tile.row0 + qbeg) * a.do_row + h0 * a.do_head;
+  const float* st = (wid == 0 ? nlse : ndelta) + (size_t)h0 * a.T + tile.row0 + qbeg;
+  const long long qwrap = a.q_head - (long long)tiles * BK * a.q_row, dwrap = a.do_head - (long long)tiles * BK * a.do_row;
+  const int swrap = a.T - tiles * BK;
   auto fetch = [&](uint32_t to) {
     const uint64_t rows = bits_below(n - fq);
     const int l = fresh_lane();
@@ -639,15 +655,14 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
       dma4(rs, (uint32_t)fresh_lane() * 4u, to + 2 * TB + wid * BK * 4);
     }
     fq += BK;
-    qs += BK * a.q_row;
-    ds += BK * a.do_row;
+    qs += sq.ldb * (BK / 2);
+    ds += sd.ldb * (BK / 2);
     st += BK;
     if (fq >= qend) {
-      const int back = fq - qbeg;
       fq = qbeg;
-      qs += a.q_head - back * a.q_row;
-      ds += a.do_head - back * a.do_row;
-      st += a.T - back;
+      qs += qwrap;
+      ds += dwrap;
+      st += swrap;
     }
   };
   if (steps) fetch(lds0);
@@ -657,9 +672,10 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
   load_frags<DP>(vf, a.v + (long long)(tile.row0 + kj) * a.v_row + kvh * a.v_head, a.dim, alive, half);
   landed(kf);
   landed(vf);
-  // (of the 128-wide head's fragments one is kept in LDS, each lane its own, and read when it is needed: in registers it is the one too many)
-  constexpr bool LENT = DP == 128;
-  if constexpr (LENT) *(LDS_PTR(bf16x8))(lds0 + 2 * SB + tid * 16) = kf[NC - 1];
+  // (of the 128-wide head's fragments the last three are kept in LDS, each lane its own, and read when they are needed: in registers they are too many)
+  constexpr int LENT = DP == 128 ? 3 : 0;
+#pragma unroll
+  for (int i = 0; i < LENT; ++i) *(LDS_PTR(bf16x8))(lds0 + 2 * SB + i * 4096 + tid * 16) = kf[NC - LENT + i];
   f32x16 gk[ND], gv[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -680,11 +696,11 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
     each<2>([&](auto qb_) {
       constexpr int qb = decltype(qb_)::value, Q = QA + qb * 32 * DP * 2, D = DA + qb * 32 * DP * 2;
       // (fragments are read DEEP - 1 ahead of their products: more do not fit)
-      constexpr int DEEP = 2;
+      constexpr int DEEP = 3;
       f.forget();
       const uint32_t stat = lds0 + 2 * TB + 16 * (fresh_lane() >> 5);
       f32x16 s, dp;
-      bf16x8 x[DEEP], kl;
+      bf16x8 x[DEEP], kl[LENT + 1];
       SCHED_FENCE();
 #pragma unroll
       for (int c = 0; c < DEEP - 1; ++c) x[c] = f.template row<Q>(c);
@@ -695,8 +711,9 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
         SCHED_FENCE();
         const int u = c + DEEP - 1;
         x[u % DEEP] = u < NC ? f.template row<Q>(u) : f.template row<D>(u - NC);
-        if (LENT && c == NC - 2) kl = *(const LDS_PTR(bf16x8))(lds0 + 2 * SB + wid * 1024 + fresh_lane() * 16);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % DEEP], LENT && c == NC - 1 ? kl : kf[c], s, 0, 0, 0);
+        const int i = c - (NC - LENT);
+        if (i + 1 >= 0 && i + 1 < LENT) kl[i + 1] = *(const LDS_PTR(bf16x8))(lds0 + 2 * SB + (i + 1) * 4096 + wid * 1024 + fresh_lane() * 16);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % DEEP], i >= 0 ? kl[i] : kf[c], s, 0, 0, 0);
       }
       SCHED_FENCE();
       if (edge) {
@@ -760,9 +777,45 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
     work(std::integral_constant<int, 0>{});
     if (left_ > 0) work(std::integral_constant<int, 1>{});
   }
+  if (to) {
+    to += tid;
+#pragma unroll
+    for (int i = 0; i < ND * 8; ++i) {
+      const f32x16& g = i < ND * 4 ? gk[i / 4] : gv[i / 4 - ND];
+      to[i * 256] = f32x4{g[(i & 3) * 4], g[(i & 3) * 4 + 1], g[(i & 3) * 4 + 2], g[(i & 3) * 4 + 3]};
+    }
+    return;
+  }
   const long long row = tile.row0 + kj;
   store_T<DP>(dk + row * a.dk_row + kvh * a.dk_head, gk, a.scale, a.dim, kj < n, half);
   store_T<DP>(dv + row * a.dv_row + kvh * a.dv_head, gv, 1.0f, a.dim, kj < n, half);
+}
+
+// The sums of the parts, in their order.  A thread has the accumulators that the same thread of the parts' workgroups left.
+template <int DP>
+__global__ __launch_bounds__(256) void attn_gqa_join_kernel(const Args a, const f32x4* __restrict__ part, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
+                                                            int split, int order) {
+  constexpr int ND = DP / 32;
+  const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % a.kv_heads, num = blockIdx.x / a.kv_heads, heads = a.heads / a.kv_heads;
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, num, order, lane);
+  if (tile.n == 0 || split_of(query_tiles(a, tile) * heads, split) == 1) return;
+  const f32x4* from = part + (size_t)blockIdx.x * split * (ND * 8 * 256) + tid;
+  const int kj = tile.first + wid * 32 + (lane & 31);
+  const long long row = tile.row0 + kj;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    f32x16 g[ND];
+#pragma unroll
+    for (int i = 0; i < ND * 4; ++i) {
+      f32x4 sum = from[(which * ND * 4 + i) * 256];
+      for (int s = 1; s < split; ++s) sum += from[(s * ND * 8 + which * ND * 4 + i) * 256];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) g[i / 4][(i & 3) * 4 + e] = sum[e];
+    }
+    if (which == 0) store_T<DP>(dk + row * a.dk_row + kvh * a.dk_head, g, a.scale, a.dim, kj < tile.n, half);
+    else store_T<DP>(dv + row * a.dv_row + kvh * a.dv_head, g, 1.0f, a.dim, kj < tile.n, half);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -800,9 +853,22 @@ Order order_of(const Args* a, bool keys) {
   return (a->right >= 0) != keys ? kUp : kDown;
 }
 
+// Tiles of the dK / dV kernel, and in how many parts it sums the heads of a group.  The chip holds 512 of its workgroups: with fewer tiles than that the
+// longest one, 4 x 2048 rows of queries at 2.9 us a step of 64 in the case above, is all that runs in the end (373 us of 600).  Two parts there: 232 and
+// 19 us for the join; four, 1888 workgroups: slower again (543 us for all against 496).
+long long units_of(const Args* a) { return ((long long)a->T / 128 + a->B) * a->kv_heads; }
+int split_for(const Args* a) {
+  const int G = a->heads / a->kv_heads;
+  int s = 1;
+  while (G % (2 * s) == 0 && units_of(a) * 2 * s <= 1024) s *= 2;
+  return s;
+}
+size_t stats_floats(const Args* a) { return ((size_t)2 * a->T * a->heads + 3) & ~(size_t)3; }  // (what is behind them starts at a multiple of 16 bytes)
+size_t part_floats(const Args* a) { return (size_t)2 * 128 * (a->dim <= 64 ? 64 : 128); }
+
 template <class K> void allow_lds(K kernel, int bytes) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 constexpr int kv_lds(int DP) { return 4 * BK * DP * 2; }
-constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4) + (DP == 128 ? 4096 : 0); }
+constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4) + (DP == 128 ? 3 * 4096 : 0); }
 void lds_limits() {
   static cocodr_lds_once once;
   if (!once.pending()) return;
@@ -827,7 +893,11 @@ extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* a, uint16_t* ctx,
   return COCODR_OK;
 }
 
-extern "C" size_t cocodr_attn_gqa_bwd_workspace_floats(const cocodr_attn_gqa_args* a) { return a && a->T > 0 && a->heads > 0 ? (size_t)2 * a->T * a->heads : 0; }
+extern "C" size_t cocodr_attn_gqa_bwd_workspace_floats(const cocodr_attn_gqa_args* a) {
+  if (!a || a->T <= 0 || a->B <= 0 || a->kv_heads <= 0 || a->heads < a->kv_heads) return 0;
+  const int split = split_for(a);
+  return stats_floats(a) + (split > 1 ? (size_t)units_of(a) * split * part_floats(a) : 0);
+}
 
 extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t* ctx, const uint16_t* dctx, const float* lse, uint16_t* dq,
                                    uint16_t* dk, uint16_t* dv, int fill, float* workspace, size_t workspace_floats, cocodr_stream_t stream) {
@@ -838,6 +908,7 @@ extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t
   CK_ARG(stride_ok(a->dq_row, a->dq_head, a->T, a->heads) && apart(a->dq_row, a->dq_head, a->T, a->heads, a->dim) && stride_ok(a->dk_row, a->dk_head, a->T, a->kv_heads) &&
              apart(a->dk_row, a->dk_head, a->T, a->kv_heads, a->dim) && stride_ok(a->dv_row, a->dv_head, a->T, a->kv_heads) && apart(a->dv_row, a->dv_head, a->T, a->kv_heads, a->dim),
          "attn_gqa_bwd: gradient strides must be multiples of 8 and keep the rows apart");
+  CK_ARG(aligned16(workspace), "attn_gqa_bwd: the workspace must be 16-byte aligned");
   if (!workspace || workspace_floats < cocodr_attn_gqa_bwd_workspace_floats(a)) {
     cocodr_set_error("attn_gqa_bwd: workspace of %zu floats is too small", workspace_floats);
     return COCODR_ERR_WORKSPACE;
@@ -845,13 +916,18 @@ extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t
   lds_limits();
   hipStream_t st = (hipStream_t)stream;
   float *ndelta = workspace, *nlse = workspace + (size_t)a->T * a->heads;
-  const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)((a->T / 128 + a->B) * a->kv_heads));
+  f32x4* part = reinterpret_cast<f32x4*>(workspace + stats_floats(a));
+  const int split = split_for(a);
+  const Order rows = order_of(a, false), keys = order_of(a, true);
+  const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)(units_of(a) * split)), gj((unsigned)units_of(a));
   if (a->dim <= 64) {
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, order_of(a, false), fill);
-    hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, order_of(a, true), fill);
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, rows, fill);
+    hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, part, split, keys, fill);
+    if (split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<64>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
   } else {
-    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, order_of(a, false), fill);
-    hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, order_of(a, true), fill);
+    hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, rows, fill);
+    hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, part, split, keys, fill);
+    if (split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<128>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
   }
   CK_LAUNCH("attn_gqa_bwd");
   return COCODR_OK;

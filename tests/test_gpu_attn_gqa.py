@@ -121,6 +121,18 @@ CASES = [
 ]
 
 
+# long and few sequences: tiles in the order of their work, the heads of a group summed in parts, one sequence far longer than the rest
+CASES += [
+    ([1500, 3, 0, 700, 64, 129], 8, 2, 64, True, (-1, -1), 0, 7, True),
+    ([3, 1500, 0, 129, 700, 64], 4, 1, 128, False, (-1, -1), 0.1, 0, True),
+    ([64, 1300, 600], 8, 1, 64, False, (-1, 40), 0, 0, False),
+    ([600, 0, 1300], 4, 2, 128, False, (40, -1), 0.3, 2, True),
+    ([1000, 1000, 1000], 2, 2, 128, True, (-1, -1), 0.2, 0, True),
+    ([257] * 63 + [300], 1, 1, 16, True, (-1, -1), 0, 0, True),
+    ([1900, 1], 8, 1, 32, True, (900, -1), 0, 0, True),
+]
+
+
 @pytest.mark.parametrize("case", CASES, ids=lambda c: f"{len(c[0])}x{max(c[0])}-h{c[1]}k{c[2]}d{c[3]}-{'causal' if c[4] else 'full'}{c[5]}-m{c[6]}")
 def test_forward_and_backward(case):
     from cocodr_amd import ops
