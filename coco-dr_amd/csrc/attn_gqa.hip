@@ -198,18 +198,19 @@ template <int DP> __device__ __forceinline__ void store_T(uint16_t* row, const f
 }
 
 // ------------------------------------------------------------------------------------------------ which rows a workgroup has
-// The tiles of TILE rows are numbered without a table: tile t of sequence b has the number off[b] / TILE + b + t.  Rounding down and
-// the + b leave a sequence at least as many numbers as it has tiles, so numbers do not collide, and there are T / TILE + B of them.
-// Number -> sequence is the last b with off[b] / TILE + b <= number: a search 64 wide, one step up to 64 sequences.
-struct Tile {
-  int n, first, row0;  // the sequence's rows (0: nothing to do), this tile's first row in it, the sequence's first row in the buffer
-};
-//
-// When sequences are long and few (by_work), the numbers go by the work of a tile instead, the most first: a workgroup with much to do that starts
+// The tiles of TILE rows are numbered without a table, and a launch has T / TILE + B workgroups, at least as many as there are tiles.
+//   up to 256 sequences: consecutive numbers in the order of the rows, from a sum over the sequences that every wave makes, four a lane; the numbers
+//     that no tile has come last, where they hold nobody up
+//   more: tile t of sequence b has the number off[b] / TILE + b + t - rounding down and the + b leave a sequence at least as many numbers as it has
+//     tiles -, and number -> sequence is the last b with off[b] / TILE + b <= number: a search 64 wide
+// When sequences are long and few, the numbers go by the work of a tile instead, the most first: a workgroup with much to do that starts
 // among the last is waited for by an empty chip.  A lane then has a sequence of c tiles.
 //   kUp, kDown: the work grows (falls) along a sequence, so tile x (tile c - 1 - x) of every sequence that has it comes before tile x - 1:
 //     x is the largest with S(x) = sum max(c - x, 0) > number, found 64 candidates at a time
 //   kLevel: it is the same along a sequence: all tiles of the longest sequence, then of the next
+struct Tile {
+  int n, first, row0;  // the sequence's rows (0: nothing to do), this tile's first row in it, the sequence's first row in the buffer
+};
 enum Order { kPlain, kUp, kDown, kLevel };
 __device__ __forceinline__ int tiles_from(int c, int B, int x) {  // S(x); x may differ from lane to lane
   int sum = 0;
@@ -218,6 +219,38 @@ __device__ __forceinline__ int tiles_from(int c, int B, int x) {  // S(x); x may
 }
 template <int TILE> __device__ __forceinline__ Tile find_tile(const int32_t* off, int B, int T, int num, int order, int lane) {
   int lo = 0, n = B, t = -1;
+  if (order == kPlain && B <= 256) {
+    const int per = (B + 63) >> 6;
+    int at[5], c[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) at[i] = min(max(i <= per ? off[min(lane * per + i, B)] : 0, 0), T);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = i < per ? (max(at[i + 1] - at[i], 0) + TILE - 1) / TILE : 0;
+      sum += c[i];
+    }
+    int upto = sum;  // the tiles of this lane's sequences and of those before
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);  // the last lane of each row of 16 to the next row
+    upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);  // lane 31 to the upper half
+    const uint64_t found = __ballot(num < upto && num >= upto - sum);
+    if (found == 0) return Tile{0, 0, 0};
+    int t = num - (upto - sum), a = at[0], e = at[1];
+    bool there = t < c[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      t -= there ? 0 : c[i - 1];
+      a = there ? a : at[i];
+      e = there ? e : at[i + 1];
+      there = there || t < c[i];
+    }
+    const int from = __builtin_amdgcn_readfirstlane(__ffsll((long long)found) - 1);
+    a = __builtin_amdgcn_readlane(a, from);
+    return Tile{__builtin_amdgcn_readlane(e, from) - a, __builtin_amdgcn_readlane(t, from) * TILE, a};
+  }
   if (order == kPlain) {
     while (n > 1) {
       const int step = (n + 63) >> 6;
@@ -336,9 +369,9 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) fill_gaps(a, ctx, lse, tid);
-  const int slots = gridDim.x / a.heads, G = a.heads / a.kv_heads;
+  const int G = a.heads / a.kv_heads;
   const int unit = blockIdx.x % a.heads, kvh = unit % a.kv_heads, h = kvh * G + unit / a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, order == kPlain ? slots - 1 - (int)(blockIdx.x / a.heads) : (int)(blockIdx.x / a.heads), order, lane);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, blockIdx.x / a.heads, order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
@@ -467,9 +500,9 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
     for (long long i = blockIdx.x; i < (long long)gap.count * a.heads; i += gridDim.x)
       if (tid * 4 < a.dim) *reinterpret_cast<uint2*>(dq + gap.row((int)(i / a.heads)) * a.dq_row + (int)(i % a.heads) * a.dq_head + tid * 4) = make_uint2(0u, 0u);
   }
-  const int slots = gridDim.x / a.heads, G = a.heads / a.kv_heads;
+  const int G = a.heads / a.kv_heads;
   const int unit = blockIdx.x % a.heads, kvh = unit % a.kv_heads, h = kvh * G + unit / a.kv_heads;
-  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, order == kPlain ? slots - 1 - (int)(blockIdx.x / a.heads) : (int)(blockIdx.x / a.heads), order, lane);
+  const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, blockIdx.x / a.heads, order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
