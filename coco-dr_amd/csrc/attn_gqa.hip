@@ -50,20 +50,6 @@ template <int DP> __device__ __forceinline__ int swz(int row) {
 }
 template <int DP> __device__ __forceinline__ int tile_off(int row, int ch) { return row * (DP * 2) + ((ch ^ swz<DP>(row)) << 4); }
 
-// operand fragment of rows r0 + (lane & 31), contraction columns 16 s + 8 (lane >> 5) .. + 7
-template <int DP> __device__ __forceinline__ bf16x8 frag_rows(const char* t, int r0, int s, int lane) {
-  return lds_read_b128(t, tile_off<DP>(r0 + (lane & 31), 2 * s + (lane >> 5)));
-}
-// operand fragment of the transposed tile: output row = column 32 dt + (lane & 31), contraction = tile rows rb + 4 (lane >> 5) + {0..3}
-// and + 8: the rows that accumulator registers 8 j .. 8 j + 7 of a 32 x 32 product hold (rb = 16 j)
-template <int DP> __device__ __forceinline__ bf16x8 frag_cols(const char* t, int rb, int dt, int lane) {
-  const int g = lane >> 4, c = lane & 15;
-  const int col = dt * 32 + ((g & 1) << 4) + ((c & 3) << 2);
-  const int row = rb + ((g >> 1) << 2) + (c >> 2);
-  const int within = (col & 7) << 1;
-  return join_tr(lds_read_tr16(t, tile_off<DP>(row, col >> 3) + within), lds_read_tr16(t, tile_off<DP>(row + 8, col >> 3) + within));
-}
-
 // 16 (4) bytes a lane from a buffer into LDS, lane-linear from `dst`.  As an asm statement, because hipcc orders every later LDS read behind the
 // builtin's vmcnt(0) - a tile on its way would be waited for in the middle of the one that is worked on.  The kernels wait themselves (dma_wait)
 // before the barrier that hands a tile over.
@@ -139,13 +125,6 @@ template <int DP> __device__ __forceinline__ void load_frags(bf16x8 (&f)[DP / 16
 template <int N> __device__ __forceinline__ void landed(bf16x8 (&f)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("s_waitcnt vmcnt(0)" : "+v"(f[i]));
-}
-
-__device__ __forceinline__ bf16x8 pack_acc(const float* p, int j) {
-  float t[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t[e] = p[j * 8 + e];
-  return as_bf16x8(pack8(t));
 }
 
 // The maximum of 2 x 16 accumulators.  fmaxf costs a quieting v_max of every operand first, so the three-operand form is written out.  Its statements
@@ -333,22 +312,45 @@ __device__ __forceinline__ uint64_t key_word(const int32_t* mask, int loaded, in
   return mask ? w & __ballot(loaded != 0) : w;
 }
 
-// LDS addresses of the fragments of a pair of tiles, in registers for the whole loop: what differs from use to use is an offset in the instruction
+// LDS addresses of the operand fragments of tiles: row(c) has rows lane & 31 of the 32 at AT, contraction columns 16 c + 8 (lane >> 5) .. + 7;
+// col(dt) is of the transposed tile: output row = column 32 dt + (lane & 31), contraction = tile rows 4 (lane >> 5) + {0..3} and + 8 behind AT, the rows
+// that accumulator registers 8 j .. 8 j + 7 of a 32 x 32 product hold (AT = row 16 j).  Here all of them in registers for the whole loop: what
+// differs from use to use is an offset in the instruction.
 template <int DP> struct Frags {
   uint32_t rows[DP / 16], cols[DP / 16];  // of row fragments 0, 1, .. and of column fragments (dt, rows 0 / 8) of a tile
-  __device__ __forceinline__ Frags(uint32_t tile_rows, uint32_t tile_cols, int lane) {
+  __device__ __forceinline__ Frags(uint32_t at, int lane) {
     const int g = lane >> 4, c = lane & 15;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-      rows[i] = tile_rows + tile_off<DP>(lane & 31, 2 * i + (lane >> 5));
+      rows[i] = at + tile_off<DP>(lane & 31, 2 * i + (lane >> 5));
       const int col = (i >> 1) * 32 + ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2) + (i & 1) * 8;
-      cols[i] = tile_cols + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
+      cols[i] = at + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
     }
   }
-  template <int ROW> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))(rows[c] + ROW * DP * 2); }
-  template <int ROW> __device__ __forceinline__ bf16x8 col(int dt) const {
-    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt] + ROW * DP * 2)),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt + 1] + ROW * DP * 2)));
+  __device__ __forceinline__ void forget() {}
+  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))(rows[c] + AT); }
+  template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt] + AT)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt + 1] + AT)));
+  }
+};
+
+// The same addresses as that of fragment 0 with a few bits flipped: a tile's rows start at multiples of DP * 2 bytes, so the chunk
+// number and its permutation are address bits of their own, and one register and an exclusive or do for eight.
+template <int DP> struct Bits {
+  uint32_t rows, cols;
+  __device__ __forceinline__ Bits(uint32_t at, int lane) {
+    const int g = lane >> 4, c = lane & 15, col = ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2);
+    rows = at + tile_off<DP>(lane & 31, lane >> 5);
+    cols = at + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
+  }
+  // what they are is forgotten: or hipcc makes the flipped addresses once, in front of the loop, and keeps each in a register of its own
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(rows), "+v"(cols)); }
+  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))((rows ^ (c << 5)) + AT); }
+  // rows + 8 flip bit 1 of the permutation (DP = 128: row bit 3 is its bit 1; DP = 64: row bit 3 its bit 1, too)
+  template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ (dt << 6)) + AT)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ ((dt << 6) | 32)) + AT + 8 * DP * 2)));
   }
 };
 
@@ -365,7 +367,7 @@ __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* l
 // A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two
 // tiles each, so that a tile is on its way while the one before is worked on.
 template <int DP>
-__global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int order, int fill) {
+__global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) fill_gaps(a, ctx, lse, tid);
@@ -386,26 +388,26 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
   constexpr int TB = BK * DP * 2, NC = DP / 16, ND = DP / 32;
   const uint32_t mine = lds_addr(smem) + wid * 1024;  // (this wave's first piece)
   const Stager<DP> sk(a.k_row, a.dim, lane, wid), sv(a.v_row, a.dim, lane, wid);
+  bf16x8 qf[NC];
+  load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
   int loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
   uint64_t word = key_word(a.mask, loaded, n, kbeg);
   loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
   sk.all(ks, mine, word);
   sv.all(vs, mine + TB, word);
 
-  bf16x8 qf[NC];
-  load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
   f32x16 o[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
   float m = kLow, l = 0.f;
-  const Frags<DP> f(lds_addr(smem), lds_addr(smem) + TB, lane);
+  std::conditional_t<DP == 64, Bits<DP>, Frags<DP>> f(lds_addr(smem), lane);
   landed(qf);
 
   // one tile of keys from k0, in buffer BUF
   auto work = [&](auto buf_, int k0) {
-    constexpr int BUF = decltype(buf_)::value, AT = BUF * 2 * BK;  // (the buffer's first row, in rows of DP)
+    constexpr int BUF = decltype(buf_)::value, KA = BUF * 2 * TB, VA = KA + TB;
     dma_wait();
     __syncthreads();
     const uint64_t now = word;
@@ -419,10 +421,11 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
       loaded = key_word_load(a.mask, tile.row0, n, k0 + 2 * BK, lane);
     }
     if (k0 >= wend || k0 + BK <= wbeg) return;
+    f.forget();
     f32x16 s[2];
     bf16x8 f0[NC], f1[NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) f0[c] = f.template row<AT>(c);
+    for (int c = 0; c < NC; ++c) f0[c] = f.template row<KA>(c);
     SCHED_FENCE();
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -430,14 +433,14 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      f1[c] = f.template row<AT + 32>(c);
+      f1[c] = f.template row<KA + TB / 2>(c);
       s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f0[c], qf[c], s[0], 0, 0, 0);
       SCHED_FENCE();
     }
     bf16x8 vf[ND];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      if (c % 2 == 0) vf[c / 2] = f.template col<AT>(c / 2);
+      if (c % 2 == 0) vf[c / 2] = f.template col<VA>(c / 2);
       s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f1[c], qf[c], s[1], 0, 0, 0);
       SCHED_FENCE();
     }
@@ -473,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_fwd_kernel(const Args a, uint
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) {
         o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], pf, o[dt], 0, 0, 0);
-        if constexpr (t < 3) vf[dt] = f.template col<AT + (t + 1) * 16>(dt);
+        if constexpr (t < 3) vf[dt] = f.template col<VA + (t + 1) * 16 * DP * 2>(dt);
       }
     });
   };
@@ -508,9 +511,12 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   const int q0 = tile.first + wid * 32, qi = q0 + (lane & 31);
   const int last = min(tile.first + 127, n - 1), wlast = min(q0 + 31, n - 1);
   const int kbeg = max(tile.first - left, 0) & ~(BK - 1), kend = min(last + right + 1, n);
-  const uint16_t* kb_ = a.k + (long long)tile.row0 * a.k_row + kvh * a.k_head;
-  const uint16_t* vb_ = a.v + (long long)tile.row0 * a.v_row + kvh * a.v_head;
+  const int wbeg = max(q0 - left, 0), wend = q0 < n ? min(wlast + right + 1, n) : 0;  // (as in the forward)
+  const int allbeg = wlast - left, allend = q0 + right + 1;
+  const uint16_t* ks = a.k + (long long)(tile.row0 + kbeg) * a.k_row + kvh * a.k_head;
+  const uint16_t* vs = a.v + (long long)(tile.row0 + kbeg) * a.v_row + kvh * a.v_head;
   const float sl2 = a.scale * kLog2e;
+  constexpr int TB = BK * DP * 2, NC = DP / 16, ND = DP / 32;
 
   bf16x8 qf[DP / 16], df[DP / 16];
   load_frags<DP>(qf, a.q + (long long)(tile.row0 + qi) * a.q_row + h * a.q_head, a.dim, qi < n, half);
@@ -545,82 +551,91 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[dt][r] = 0.f;
 
-  constexpr int TB = BK * DP * 2;
   const uint32_t lds0 = lds_addr(smem) + wid * 1024;  // (this wave's first piece)
   const Stager<DP> sk(a.k_row, a.dim, lane, wid), sv(a.v_row, a.dim, lane, wid);
   int loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
   uint64_t word = key_word(a.mask, loaded, n, kbeg);
   loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
-  if (kbeg < kend) {
-    sk.all(kb_ + kbeg * a.k_row, lds0, word);
-    sv.all(vb_ + kbeg * a.v_row, lds0 + TB, word);
-  }
-  int buf = 0;
-  for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
-    const char* Kt = smem + buf * 2 * TB;
-    const char* Vt = Kt + TB;
+  sk.all(ks, lds0, word);
+  sv.all(vs, lds0 + TB, word);
+  Bits<DP> f(lds_addr(smem), lane);
+  // one tile of keys from k0, in buffer BUF
+  auto work = [&](auto buf_, int k0) {
+    constexpr int BUF = decltype(buf_)::value;
     dma_wait();
     __syncthreads();
-    const uint64_t next = key_word(a.mask, loaded, n, k0 + BK);
+    const uint64_t now = word;
     if (k0 + BK < kend) {
-      const uint32_t to = lds0 + (buf ^ 1) * 2 * TB;
-      sk.all(kb_ + (long long)(k0 + BK) * a.k_row, to, next);
-      sv.all(vb_ + (long long)(k0 + BK) * a.v_row, to + TB, next);
+      word = key_word(a.mask, loaded, n, k0 + BK);
+      const uint32_t to = lds0 + (BUF ^ 1) * 2 * TB;
+      ks += BK * a.k_row;
+      vs += BK * a.v_row;
+      sk.all(ks, to, word);
+      sv.all(vs, to + TB, word);
       loaded = key_word_load(a.mask, tile.row0, n, k0 + 2 * BK, lane);
     }
-    const uint64_t now = word;
-    word = next;
-    if (q0 >= n || k0 > wlast + right || k0 + BK <= q0 - left || now == 0) continue;
-    const bool edge = now != ~0ull || k0 < wlast - left || k0 + BK > q0 + right + 1;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    if (k0 >= wend || k0 + BK <= wbeg) return;
+    const bool edge = now != ~0ull || k0 < allbeg || k0 + BK > allend;
+    each<2>([&](auto kb_) {
+      // (fragments are read DEEP - 1 ahead of their products)
+      constexpr int kb = decltype(kb_)::value, K = BUF * 2 * TB + kb * TB / 2, V = K + TB, DEEP = 3;
+      f.forget();
       f32x16 s, dp;
+      bf16x8 x[DEEP], z[DEEP];
+      SCHED_FENCE();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = nd; }
+      for (int c = 0; c < DEEP - 1; ++c) x[c] = f.template row<K>(c);
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) {
-        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows<DP>(Kt, kb * 32, c, lane), qf[c], s, 0, 0, 0);
-        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows<DP>(Vt, kb * 32, c, lane), df[c], dp, 0, 0, 0);
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = nd; }  // dP starts at -delta
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        SCHED_FENCE();
+        const int u = c + DEEP - 1;
+        x[u % DEEP] = u < NC ? f.template row<K>(u) : f.template row<V>(u - NC);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % DEEP], qf[c], s, 0, 0, 0);
       }
-      float ds[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sl2, nl)) * dp[r];
+      SCHED_FENCE();
       if (edge) {
         const int base = k0 + kb * 32;
         const uint32_t see = (bits32(qi - left - base, qi + right + 1 - base) & (uint32_t)(now >> (kb * 32))) >> (4 * half);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? ds[r] : 0.f;
+        for (int r = 0; r < 16; ++r) s[r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
       }
+      // beside the products of dP: the probabilities
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        SCHED_FENCE();
+        const int u = c + DEEP - 1;
+        if (u < NC) x[(NC + u) % DEEP] = f.template row<V>(u);
+        dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[(NC + c) % DEEP], df[c], dp, 0, 0, 0);
+#pragma unroll
+        for (int e = c * 16 / NC; e < (c + 1) * 16 / NC; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sl2, nl));
+      }
+      SCHED_FENCE();
+      each<DEEP - 1>([&](auto k) { z[decltype(k)::value] = f.template col<K + decltype(k)::value / ND * 16 * DP * 2>(decltype(k)::value % ND); });
+      bf16x8 pf[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const bf16x8 f = pack_acc(ds, j);
+        float d[8];
 #pragma unroll
-        for (int dt = 0; dt < DP / 32; ++dt)
-          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_cols<DP>(Kt, kb * 32 + j * 16, dt, lane), f, acc[dt], 0, 0, 0);
+        for (int e = 0; e < 8; ++e) d[e] = s[j * 8 + e] * dp[j * 8 + e];
+        pf[j] = as_bf16x8(pack8(d));
       }
-    }
+      each<2 * ND>([&](auto k_) {
+        constexpr int k = decltype(k_)::value, u = k + DEEP - 1;
+        SCHED_FENCE();
+        if constexpr (u < 2 * ND) z[u % DEEP] = f.template col<K + u / ND * 16 * DP * 2>(u % ND);
+        acc[k % ND] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(z[k % DEEP], pf[k / ND], acc[k % ND], 0, 0, 0);
+      });
+      SCHED_FENCE();
+    });
+  };
+  for (int k0 = kbeg; k0 < kend; k0 += 2 * BK) {
+    work(std::integral_constant<int, 0>{}, k0);
+    if (k0 + BK < kend) work(std::integral_constant<int, 1>{}, k0 + BK);
   }
   store_T<DP>(dq + (long long)(tile.row0 + qi) * a.dq_row + h * a.dq_head, acc, a.scale, a.dim, qi < n, half);
 }
-
-// LDS address of a fragment as the address of fragment 0 with a few bits flipped: a tile's rows start at multiples of DP * 2 bytes, so the chunk
-// number and its permutation are address bits of their own, and one register and an exclusive or do for eight.
-template <int DP> struct Bits {
-  uint32_t rows, cols;
-  __device__ __forceinline__ Bits(uint32_t at, int lane) {
-    const int g = lane >> 4, c = lane & 15, col = ((g & 1) << 4) + ((c & 3) << 2), row = ((g >> 1) << 2) + (c >> 2);
-    rows = at + tile_off<DP>(lane & 31, lane >> 5);
-    cols = at + tile_off<DP>(row, col >> 3) + ((col & 7) << 1);
-  }
-  // what they are is forgotten: or hipcc makes the flipped addresses once, in front of the loop, and keeps each in a register of its own
-  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(rows), "+v"(cols)); }
-  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))((rows ^ (c << 5)) + AT); }
-  // rows + 8 flip bit 1 of the permutation (DP = 128: row bit 3 is its bit 1; DP = 64: row bit 3 its bit 1, too)
-  template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
-    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ (dt << 6)) + AT)),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ ((dt << 6) | 32)) + AT + 8 * DP * 2)));
-  }
-};
 
 // the tiles of queries that see a tile of 128 keys, and in how many parts a group's heads are summed for it
 __device__ __forceinline__ int query_tiles(const Args& a, const Tile& t) {
