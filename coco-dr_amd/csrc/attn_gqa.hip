@@ -202,7 +202,9 @@ template <int TILE> __device__ __forceinline__ Tile find_tile(const int32_t* off
     const int per = (B + 63) >> 6;
     int at[5], c[4], sum = 0;
 #pragma unroll
-    for (int i = 0; i < 5; ++i) at[i] = min(max(i <= per ? off[min(lane * per + i, B)] : 0, 0), T);
+    for (int i = 0; i < 5; ++i) at[i] = off[min(lane * per + i, B)];  // (all five always: a condition would have them wait for one another)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) at[i] = min(max(at[i], 0), T);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       c[i] = i < per ? (max(at[i + 1] - at[i], 0) + TILE - 1) / TILE : 0;
@@ -302,6 +304,14 @@ __device__ __forceinline__ uint32_t bits32(int lo, int hi) {
   return below_hi & ~below_lo;
 }
 __device__ __forceinline__ uint64_t bits_below(int n) { return n >= 64 ? ~0ull : (n <= 0 ? 0ull : (1ull << n) - 1ull); }
+
+// v where bit AT of `see` is set, -inf where it is not: two instructions (hipcc's own choice is a test, a wait state and a selection, 40 % of a
+// masked tile's instructions)
+template <int AT> __device__ __forceinline__ float seen(uint32_t see, float v) {
+  uint32_t all;
+  asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(all) : "v"(see), "n"(AT));
+  return __uint_as_float((__float_as_uint(v) & all) | (__float_as_uint(-INFINITY) & ~all));
+}
 
 // which of the BK keys from k0 on exist and are not masked out.  The load is started (key_word_load) one tile before its ballot is taken.
 __device__ __forceinline__ int key_word_load(const int32_t* mask, int row0, int n, int k0, int lane) {
@@ -449,19 +459,23 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(con
       for (int kb = 0; kb < 2; ++kb) {
         const int base = k0 + kb * 32;
         const uint32_t see = (bits32(qi - left - base, qi + right + 1 - base) & (uint32_t)(now >> (kb * 32))) >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[kb][r] : -INFINITY;
+        each<16>([&](auto r_) {
+          constexpr int r = decltype(r_)::value;
+          s[kb][r] = seen<8 * (r >> 2) + (r & 3)>(see, s[kb][r]);
+        });
       }
     }
     const float top = max_halves(max32(s)) * sl2;
     if (__any(top > m + kGrow)) {
       const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - up);
       m = up;
-      l *= f;
+      if (__any(l != 0.f)) {  // (or the sums are zeros: nothing to scale)
+        l *= f;
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
+        for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+          for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+      }
     }
     // P of a 16-key step is made while the products of the step before run; the step's rows of V are fetched one step ahead
     each<4>([&](auto t_) {
@@ -598,8 +612,10 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
       if (edge) {
         const int base = k0 + kb * 32;
         const uint32_t see = (bits32(qi - left - base, qi + right + 1 - base) & (uint32_t)(now >> (kb * 32))) >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+        each<16>([&](auto r_) {
+          constexpr int r = decltype(r_)::value;
+          s[r] = seen<8 * (r >> 2) + (r & 3)>(see, s[r]);
+        });
       }
       // beside the products of dP: the probabilities
 #pragma unroll
@@ -767,8 +783,10 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
       if (edge) {
         const int l = fresh_lane(), key = key0 + (l & 31), base = at + qb * 32;
         const uint32_t see = (live >> (l & 31)) & 1 ? bits32(key - right - base, min(key + left + 1, n) - base) >> (4 * (l >> 5)) : 0u;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = (see >> (8 * (r >> 2) + (r & 3))) & 1 ? s[r] : -INFINITY;
+        each<16>([&](auto r_) {
+          constexpr int r = decltype(r_)::value;
+          s[r] = seen<8 * (r >> 2) + (r & 3)>(see, s[r]);
+        });
       }
       SCHED_FENCE();
 #pragma unroll
