@@ -60,6 +60,7 @@ __device__ __forceinline__ rsrc_t rsrc_of(const void* base, uint32_t bytes) {
 }
 // scalars that a vector instruction wrote may be read by a memory instruction five states later, and hipcc does not look into dma16
 __device__ __forceinline__ void rsrc_settled(rsrc_t a) { asm volatile("s_nop 4" ::"s"(a)); }
+template <class V> __device__ __forceinline__ LDS_PTR(V) lds_at(uint32_t addr) { return (LDS_PTR(V))(uintptr_t)addr; }
 __device__ __forceinline__ uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(LDS_PTR(const void))p; }
 __device__ __forceinline__ void dma16(rsrc_t rs, uint32_t off, uint32_t more, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(off), "s"(rs), "s"(more), "s"(dst) : "memory", "m0");
@@ -338,10 +339,10 @@ template <int DP> struct Frags {
     }
   }
   __device__ __forceinline__ void forget() {}
-  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))(rows[c] + AT); }
+  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *lds_at<const bf16x8>(rows[c] + AT); }
   template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
-    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt] + AT)),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))(cols[2 * dt + 1] + AT)));
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(cols[2 * dt] + AT)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>(cols[2 * dt + 1] + AT)));
   }
 };
 
@@ -356,11 +357,11 @@ template <int DP> struct Bits {
   }
   // what they are is forgotten: or hipcc makes the flipped addresses once, in front of the loop, and keeps each in a register of its own
   __device__ __forceinline__ void forget() { asm volatile("" : "+v"(rows), "+v"(cols)); }
-  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *(const LDS_PTR(bf16x8))((rows ^ (c << 5)) + AT); }
+  template <int AT> __device__ __forceinline__ bf16x8 row(int c) const { return *lds_at<const bf16x8>((rows ^ (c << 5)) + AT); }
   // rows + 8 flip bit 1 of the permutation (DP = 128: row bit 3 is its bit 1; DP = 64: row bit 3 its bit 1, too)
   template <int AT> __device__ __forceinline__ bf16x8 col(int dt) const {
-    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ (dt << 6)) + AT)),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((LDS_PTR(s16x4))((cols ^ ((dt << 6) | 32)) + AT + 8 * DP * 2)));
+    return join_tr(__builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>((cols ^ (dt << 6)) + AT)),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<s16x4>((cols ^ ((dt << 6) | 32)) + AT + 8 * DP * 2)));
   }
 };
 
@@ -739,7 +740,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
   // (of the 128-wide head's fragments the last three are kept in LDS, each lane its own, and read when they are needed: in registers they are too many)
   constexpr int LENT = DP == 128 ? 3 : 0;
 #pragma unroll
-  for (int i = 0; i < LENT; ++i) *(LDS_PTR(bf16x8))(lds0 + 2 * SB + i * 4096 + tid * 16) = kf[NC - LENT + i];
+  for (int i = 0; i < LENT; ++i) *lds_at<bf16x8>(lds0 + 2 * SB + i * 4096 + tid * 16) = kf[NC - LENT + i];
   f32x16 gk[ND], gv[ND];
 #pragma unroll
   for (int dt = 0; dt < ND; ++dt)
@@ -776,7 +777,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
         const int u = c + DEEP - 1;
         x[u % DEEP] = u < NC ? f.template row<Q>(u) : f.template row<D>(u - NC);
         const int i = c - (NC - LENT);
-        if (i + 1 >= 0 && i + 1 < LENT) kl[i + 1] = *(const LDS_PTR(bf16x8))(lds0 + 2 * SB + (i + 1) * 4096 + wid * 1024 + fresh_lane() * 16);
+        if (i + 1 >= 0 && i + 1 < LENT) kl[i + 1] = *lds_at<const bf16x8>(lds0 + 2 * SB + (i + 1) * 4096 + wid * 1024 + fresh_lane() * 16);
         s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[c % DEEP], i >= 0 ? kl[i] : kf[c], s, 0, 0, 0);
       }
       SCHED_FENCE();
@@ -791,7 +792,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
       SCHED_FENCE();
 #pragma unroll
       for (int rg = 0; rg < 4; ++rg) {  // dP starts at -delta of its rows
-        const f32x4 d4 = *(const LDS_PTR(f32x4))(stat + decltype(buf_)::value * SB + BK * 4 + qb * 128 + 32 * rg);
+        const f32x4 d4 = *lds_at<const f32x4>(stat + decltype(buf_)::value * SB + BK * 4 + qb * 128 + 32 * rg);
         dp[rg * 4] = d4[0]; dp[rg * 4 + 1] = d4[1]; dp[rg * 4 + 2] = d4[2]; dp[rg * 4 + 3] = d4[3];
       }
       // beside the products of dP: the probabilities, two registers a product
@@ -804,7 +805,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
         dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[(NC + c) % DEEP], vf[c], dp, 0, 0, 0);
 #pragma unroll
         for (int e = c * 16 / NC; e < (c + 1) * 16 / NC; ++e) {
-          if (e % 4 == 0) l4 = *(const LDS_PTR(f32x4))(stat + decltype(buf_)::value * SB + qb * 128 + 8 * e);
+          if (e % 4 == 0) l4 = *lds_at<const f32x4>(stat + decltype(buf_)::value * SB + qb * 128 + 8 * e);
           s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sl2, l4[e % 4]));
         }
       }
