@@ -933,6 +933,13 @@ int split_for(const Args* a) {
 size_t stats_floats(const Args* a) { return ((size_t)2 * a->T * a->heads + 3) & ~(size_t)3; }  // (what is behind them starts at a multiple of 16 bytes)
 size_t part_floats(const Args* a) { return (size_t)2 * 128 * (a->dim <= 64 ? 64 : 128); }
 
+// the strides between the rows of a single row may be anything, and the kernels' tiles reach as far as 64 strides
+Args tidy(const Args* a) {
+  Args b = *a;
+  if (b.T == 1) b.q_row = b.k_row = b.v_row = b.o_row = b.do_row = b.dq_row = b.dk_row = b.dv_row = 0;
+  return b;
+}
+
 template <class K> void allow_lds(K kernel, int bytes) { (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 constexpr int kv_lds(int DP) { return 4 * BK * DP * 2; }
 constexpr int qd_lds(int DP) { return 2 * (2 * BK * DP * 2 + 2 * BK * 4) + (DP == 128 ? 3 * 4096 : 0); }
@@ -947,8 +954,9 @@ void lds_limits() {
 
 }  // namespace
 
-extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* a, uint16_t* ctx, float* lse, int fill, cocodr_stream_t stream) {
-  if (int rc = check(a, "attn_gqa_fwd")) return rc;
+extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* args, uint16_t* ctx, float* lse, int fill, cocodr_stream_t stream) {
+  if (int rc = check(args, "attn_gqa_fwd")) return rc;
+  const Args b = tidy(args), *a = &b;
   CK_ARG(ctx && lse && aligned16(ctx), "attn_gqa_fwd: ctx and lse must be given, ctx 16-byte aligned");
   CK_ARG(stride_ok(a->o_row, a->o_head, a->T, a->heads) && apart(a->o_row, a->o_head, a->T, a->heads, a->dim), "attn_gqa_fwd: ctx strides must be multiples of 8 and keep its rows apart");
   lds_limits();
@@ -966,9 +974,10 @@ extern "C" size_t cocodr_attn_gqa_bwd_workspace_floats(const cocodr_attn_gqa_arg
   return stats_floats(a) + (split > 1 ? (size_t)units_of(a) * split * part_floats(a) : 0);
 }
 
-extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* a, const uint16_t* ctx, const uint16_t* dctx, const float* lse, uint16_t* dq,
+extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* args, const uint16_t* ctx, const uint16_t* dctx, const float* lse, uint16_t* dq,
                                    uint16_t* dk, uint16_t* dv, int fill, float* workspace, size_t workspace_floats, cocodr_stream_t stream) {
-  if (int rc = check(a, "attn_gqa_bwd")) return rc;
+  if (int rc = check(args, "attn_gqa_bwd")) return rc;
+  const Args b = tidy(args), *a = &b;
   CK_ARG(ctx && dctx && lse && dq && dk && dv, "attn_gqa_bwd: null pointer");
   CK_ARG(aligned16(ctx) && aligned16(dctx) && aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_gqa_bwd: tensors must be 16-byte aligned");
   CK_ARG(stride_ok(a->o_row, a->o_head, a->T, a->heads) && stride_ok(a->do_row, a->do_head, a->T, a->heads), "attn_gqa_bwd: strides must be multiples of 8 elements, rows less than 2^23 apart");

@@ -45,6 +45,9 @@ def test_outputs_that_overlap_or_are_missing(lib):  # noqa: F811
     a = args()
     need = lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(a))
     assert need >= 2 * 100 * 8
+    assert bwd(ws=4104) == -1 and b"workspace" in lib.cocodr_last_error()
+    # few tiles of a group of query heads: room for the parts of dk and dv, 2 x 128 x 64 floats a tile and part
+    assert lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(args(heads=16))) >= 2 * 100 * 16 + 2 * (100 // 128 + 3) * 4 * 2 * 128 * 64
     assert bwd(floats=need - 1) == -3 and b"workspace" in lib.cocodr_last_error() and bwd(ws=0) == -3
 
 

@@ -116,6 +116,8 @@ CASES = [
     ([333, 260], 2, 1, 64, False, (20, -1), 0.9, 0, False),
     ([1100], 8, 2, 128, True, (-1, -1), 0, 0, True),
     ([40] * 70 + [3] * 70, 1, 1, 64, True, (-1, -1), 0, 9, True),   # more than 64 sequences: the search for a tile's sequence takes two steps
+    ([5] * 256, 1, 1, 32, True, (-1, -1), 0.1, 0, True),             # 256: the most that are numbered without gaps
+    ([130, 5] * 128 + [1], 1, 1, 32, False, (-1, -1), 0, 3, True),
     ([2] * 4200, 1, 1, 32, False, (-1, -1), 0, 0, True),            # ... three
     ([256, 128], 32, 8, 72, True, (-1, -1), 0, 0, True),
 ]
@@ -219,6 +221,19 @@ def test_row_offsets_behind_two_gib():
     a, b = ops.attn_gqa_fwd(q, k, v, off, causal=True), ops.attn_gqa_fwd(sq, sk, sv, off, causal=True)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     ga, gb = (ops.attn_gqa_bwd(*t, a[0], dctx, a[1], off, causal=True) for t in ((q, k, v), (sq, sk, sv)))
+    assert all(torch.equal(x, y) for x, y in zip(ga, gb))
+
+
+@pytest.mark.parametrize("stride", [7, 8, 1 << 24, 1 << 31])
+def test_a_single_row_with_any_stride(stride):
+    """what stands between the rows of one row does not count, whatever a view says it is"""
+    from cocodr_amd import ops
+    q, k, v, dctx, off = make([1], 4, 2, 128, seed=14, fused=False)
+    q, k, v, dctx = (t.contiguous() for t in (q, k, v, dctx))
+    odd = [torch.as_strided(t, t.shape, (stride, 128, 1)) for t in (q, k, v, dctx)]
+    a, b = ops.attn_gqa_fwd(q, k, v, off), ops.attn_gqa_fwd(*odd[:3], off)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    ga, gb = (ops.attn_gqa_bwd(*t[:3], a[0], t[3], a[1], off) for t in ((q, k, v, dctx), odd))
     assert all(torch.equal(x, y) for x, y in zip(ga, gb))
 
 
