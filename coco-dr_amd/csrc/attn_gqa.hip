@@ -505,8 +505,14 @@ __global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(con
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+// how many keys row i of a sequence sees, masked ones among them
+__device__ __forceinline__ int keys_of(int i, int n, int left, int right) { return min(i + right, n - 1) - max(i - left, 0) + 1; }
+
 // dQ: 128 query rows of one head a workgroup, 32 a wave (lane = query), over tiles of 64 keys as in the forward.  A wave has its rows of dO in
 // registers: with ctx beside them it also makes -delta and -lse (in log2 units) of its rows and leaves them, [heads][T] each, for the dK / dV kernel.
+// ctx is rounded to bf16, and so is off by 2^-9 of itself, rms, against dP of which it is the mean: nothing beside the rounding of dS where a row sees
+// many keys, but up to twice its effect where it sees a few.  Workgroups with a row of up to 64 keys take delta = sum p dp from a pass of their own over
+// their few tiles instead of from ctx (sequences of 1 to 2048, dq off by 2.6e-3 in norm with ctx).
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,
                                                              const float* __restrict__ lse, float* __restrict__ ndelta, float* __restrict__ nlse,
@@ -528,8 +534,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   const int kbeg = max(tile.first - left, 0) & ~(BK - 1), kend = min(last + right + 1, n);
   const int wbeg = max(q0 - left, 0), wend = q0 < n ? min(wlast + right + 1, n) : 0;  // (as in the forward)
   const int allbeg = wlast - left, allend = q0 + right + 1;
-  const uint16_t* ks = a.k + (long long)(tile.row0 + kbeg) * a.k_row + kvh * a.k_head;
-  const uint16_t* vs = a.v + (long long)(tile.row0 + kbeg) * a.v_row + kvh * a.v_head;
+  const uint16_t *ks, *vs;
   const float sl2 = a.scale * kLog2e;
   constexpr int TB = BK * DP * 2, NC = DP / 16, ND = DP / 32;
 
@@ -541,7 +546,8 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   float nl = qi < n ? (lse[at] == -INFINITY ? -INFINITY : -lse[at] * kLog2e) : 0.f;
   asm volatile("s_waitcnt vmcnt(0)" : "+v"(nl));
   float nd = 0.f;
-  {
+  const int few = min(keys_of(tile.first, n, left, right), keys_of(last, n, left, right));
+  if (few > 64) {
     bf16x8 of[DP / 16];
     load_frags<DP>(of, ctx + (long long)(tile.row0 + qi) * a.o_row + h * a.o_head, a.dim, qi < n, half);
 #pragma unroll
@@ -556,10 +562,6 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
   }
   landed(qf);
   landed(df);
-  if (qi < n && lane < 32) {
-    ndelta[at] = nd;
-    nlse[at] = nl;
-  }
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
@@ -568,15 +570,24 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
 
   const uint32_t lds0 = lds_addr(smem) + wid * 1024;  // (this wave's first piece)
   const Stager<DP> sk(a.k_row, a.dim, lane, wid), sv(a.v_row, a.dim, lane, wid);
-  int loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
-  uint64_t word = key_word(a.mask, loaded, n, kbeg);
-  loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
-  sk.all(ks, lds0, word);
-  sv.all(vs, lds0 + TB, word);
+  int loaded;
+  uint64_t word;
+  auto first_tile = [&]() {
+    loaded = key_word_load(a.mask, tile.row0, n, kbeg, lane);
+    word = key_word(a.mask, loaded, n, kbeg);
+    loaded = key_word_load(a.mask, tile.row0, n, kbeg + BK, lane);
+    ks = a.k + (long long)(tile.row0 + kbeg) * a.k_row + kvh * a.k_head;
+    vs = a.v + (long long)(tile.row0 + kbeg) * a.v_row + kvh * a.v_head;
+    sk.all(ks, lds0, word);
+    sv.all(vs, lds0 + TB, word);
+  };
+  first_tile();
+  float sum = 0.f;
   Bits<DP> f(lds_addr(smem), lane);
-  // one tile of keys from k0, in buffer BUF
-  auto work = [&](auto buf_, int k0) {
+  // one tile of keys from k0, in buffer BUF; DELTA: only its share of delta
+  auto work = [&](auto buf_, auto delta_, int k0) {
     constexpr int BUF = decltype(buf_)::value;
+    constexpr bool DELTA = decltype(delta_)::value;
     dma_wait();
     __syncthreads();
     const uint64_t now = word;
@@ -601,7 +612,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
 #pragma unroll
       for (int c = 0; c < DEEP - 1; ++c) x[c] = f.template row<K>(c);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = nd; }  // dP starts at -delta
+      for (int r = 0; r < 16; ++r) { s[r] = 0.f; dp[r] = DELTA ? 0.f : nd; }  // dP starts at -delta
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         SCHED_FENCE();
@@ -629,6 +640,11 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
         for (int e = c * 16 / NC; e < (c + 1) * 16 / NC; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], sl2, nl));
       }
       SCHED_FENCE();
+      if constexpr (DELTA) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum = fmaf(s[e], dp[e], sum);
+        return;
+      }
       each<DEEP - 1>([&](auto k) { z[decltype(k)::value] = f.template col<K + decltype(k)::value / ND * 16 * DP * 2>(decltype(k)::value % ND); });
       bf16x8 pf[2];
 #pragma unroll
@@ -647,10 +663,23 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
       SCHED_FENCE();
     });
   };
-  for (int k0 = kbeg; k0 < kend; k0 += 2 * BK) {
-    work(std::integral_constant<int, 0>{}, k0);
-    if (k0 + BK < kend) work(std::integral_constant<int, 1>{}, k0 + BK);
+  auto pass = [&](auto delta) {
+    for (int k0 = kbeg; k0 < kend; k0 += 2 * BK) {
+      work(std::integral_constant<int, 0>{}, delta, k0);
+      if (k0 + BK < kend) work(std::integral_constant<int, 1>{}, delta, k0 + BK);
+    }
+  };
+  if (few <= 64) {
+    pass(std::true_type{});
+    nd = -sum_halves(sum);
+    __syncthreads();
+    first_tile();
   }
+  if (qi < n && lane < 32) {
+    ndelta[at] = nd;
+    nlse[at] = nl;
+  }
+  pass(std::false_type{});
   store_T<DP>(dq + (long long)(tile.row0 + qi) * a.dq_row + h * a.dq_head, acc, a.scale, a.dim, qi < n, half);
 }
 
