@@ -375,8 +375,14 @@ __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* l
   }
 }
 
-// A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two
-// tiles each, so that a tile is on its way while the one before is worked on.
+// A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two tiles each, so that
+// a tile is on its way while the one before is worked on.  Scores, statistics and the output never leave the registers: one pass over the keys.
+// Heads of 128, long sequences: bound by the matrix pipe, and that by power: 8192 causal, 32 / 8 heads, 570 us = 965 TFLOP/s, where the pipe is 48 % busy
+// at 1.9 GHz; 64 rows a wave (one wave a SIMD, half the LDS traffic) took 580 us at 2.4 GHz, eight waves sharing a tile 571.  So 32 rows and two
+// workgroups a CU, which short sequences want too (129 against 84 us with eight waves, 256 sequences of 20 to 256).
+// Heads of 64, short sequences: bound by what stands before the first product - offsets, mask, first tile, each waiting for the one before, 5 of a
+// workgroup's 10 us - so as many workgroups at once as registers allow (122: four a CU; addresses by flipped bits instead of a register each): 256
+// sequences of 20 to 256, 16 heads, masked: 71 us, 2.7 TB/s.  Two heads after one another in a workgroup saved nothing (71 - 75 us).
 template <int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -512,7 +518,8 @@ __device__ __forceinline__ int keys_of(int i, int n, int left, int right) { retu
 // registers: with ctx beside them it also makes -delta and -lse (in log2 units) of its rows and leaves them, [heads][T] each, for the dK / dV kernel.
 // ctx is rounded to bf16, and so is off by 2^-9 of itself, rms, against dP of which it is the mean: nothing beside the rounding of dS where a row sees
 // many keys, but up to twice its effect where it sees a few.  Workgroups with a row of up to 64 keys take delta = sum p dp from a pass of their own over
-// their few tiles instead of from ctx (sequences of 1 to 2048, dq off by 2.6e-3 in norm with ctx).
+// their few tiles instead of from ctx (16 sequences of 1 to 2048: dq off by 2.4e-3 in norm, 2.6e-3 with ctx; short ones alone 2.3e-3 and 4e-3).
+// 4 x 4096 causal, 32 / 8 heads of 128: 765 - 830 us, 3 products of 275 GFLOP, 1.0 PFLOP/s: power again.  64 x 128, 12 heads of 64: 20 us, 76 MB at 3.8 TB/s.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,
                                                              const float* __restrict__ lse, float* __restrict__ ndelta, float* __restrict__ nlse,
@@ -695,7 +702,12 @@ constexpr int kWhole = 48;
 __device__ __forceinline__ int split_of(int steps, int split) { return steps > kWhole ? split : 1; }
 
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows.  The wave's
-// K and V fragments and its 128 accumulators stay in registers: 256 of them are just enough, and leave room for a second wave on the SIMD.
+// K and V fragments and its 128 accumulators stay in registers: 256 of them are just enough, and leave room for a second wave on the SIMD.  The second
+// wave is what it takes: alone on its SIMD a wave issues an instruction every 4.8 clocks and waits 8 for a result, and the kernel took 1561 us for
+// 4 x 4096 causal, 32 / 8 heads of 128; with two it takes 1010 - 1094, 4 products of 275 GFLOP, 1.05 PFLOP/s.  What it costs: addresses made by flipping
+// bits, fragments fetched two products ahead and not more, three of K's in LDS, the probabilities two registers at a time beside dP's products.
+// 64 x 128, 12 heads of 64: 21 us, 76 MB at 3.6 TB/s.  (One kernel for dQ, dK and dV of such short sequences, dS through LDS: 31 us + 4 for the
+// other's empty launch, against 20 + 21; with registers for it, windows over long sequences lost as much as it won.)
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,

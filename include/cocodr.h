@@ -179,7 +179,8 @@ int cocodr_attn_bwd_drop(const uint16_t* qkv, const int32_t* mask, const uint16_
  * sees its keys j with i - left <= j <= i + right (-1: no limit; causal = right 0) whose mask entry (int32 [T], NULL: all) is not 0.
  *   ctx_i = sum_j softmax_j(scale q_i . k_j) v_j [T, heads, dim] bf16, lse [heads, T] fp32 = log sum_j exp(scale q_i . k_j);
  *   a row that sees nothing gets ctx = 0, lse = -inf and zero gradients.  K and V rows behind a sequence or masked out are not read
- *   (they may hold anything, NaN too).
+ *   (they may hold anything, NaN too); keys that a row does not see because of causality or its window count as 0 times their values, so
+ *   the others have to be finite.
  * fill: rows that belong to no sequence get ctx = 0 and lse = -inf, zero gradients (1), or are left as they are (0).
  * Backward: recomputes the probabilities from q, k and lse; dk and dv sum over the query heads of a key head's group.  No atomics:
  * the same inputs give the same bits.  workspace: cocodr_attn_gqa_bwd_workspace_floats(args) floats, 16-byte aligned.
