@@ -612,6 +612,8 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const
     each<2>([&](auto kb_) {
       // (fragments are read DEEP - 1 ahead of their products)
       constexpr int kb = decltype(kb_)::value, K = BUF * 2 * TB + kb * TB / 2, V = K + TB, DEEP = 3;
+      // (none of these 32 is seen: 1 % of 4 x 4096 causal with heads of 128.  With heads of 64 the branch costs 64 x 128 rows as much as it saves a window.)
+      if (DP == 128 && (k0 + kb * 32 >= wend || k0 + kb * 32 + 32 <= wbeg)) return;
       f.forget();
       f32x16 s, dp;
       bf16x8 x[DEEP], z[DEEP];
@@ -801,6 +803,8 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
     const bool edge = live != ~0u || at < wlast - right || at + BK > key0 + left + 1;
     each<2>([&](auto qb_) {
       constexpr int qb = decltype(qb_)::value, Q = QA + qb * 32 * DP * 2, D = DA + qb * 32 * DP * 2;
+      // (none of these 32 sees a key of the wave; as in dQ)
+      if (DP == 128 && (at + qb * 32 >= qend || at + qb * 32 > wlast + left || at + qb * 32 + 32 <= key0 - right)) return;
       // (fragments are read DEEP - 1 ahead of their products: more do not fit)
       constexpr int DEEP = 3;
       f.forget();
