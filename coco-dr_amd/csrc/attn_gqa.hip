@@ -180,7 +180,8 @@ template <int DP> __device__ __forceinline__ void store_T(uint16_t* row, const f
 // ------------------------------------------------------------------------------------------------ which rows a workgroup has
 // The tiles of TILE rows are numbered without a table, and a launch has T / TILE + B workgroups, at least as many as there are tiles.
 //   up to 256 sequences: consecutive numbers in the order of the rows, from a sum over the sequences that every wave makes, four a lane; the numbers
-//     that no tile has come last, where they hold nobody up
+//     that no tile has come last, where they hold nobody up (64 x 128 rows, 12 heads, forward and backward: 58 us; 75 with the numbers below, every
+//     second of which is empty there)
 //   more: tile t of sequence b has the number off[b] / TILE + b + t - rounding down and the + b leave a sequence at least as many numbers as it has
 //     tiles -, and number -> sequence is the last b with off[b] / TILE + b <= number: a search 64 wide
 // When sequences are long and few, the numbers go by the work of a tile instead, the most first: a workgroup with much to do that starts
@@ -958,7 +959,8 @@ int check(const Args* a, const char* what) {
 }
 
 // by work: where tiles have so much of it (sequences of 256 rows and more on average) that the longer search for them does not count, where their work
-// differs (no window on both sides), and where a lane each does for the sequences
+// differs (no window on both sides), and where a lane each does for the sequences.  Forward and backward, 32 / 8 heads of 128, causal: 4 x 4096 2393 us by
+// work, 2690 in the order of the rows; 16 sequences of 1 to 2048 600 and 610.
 Order order_of(const Args* a, bool keys) {
   if (a->B > 64 || a->T / a->B < 256 || (a->left >= 0 && a->right >= 0)) return kPlain;
   if (a->left < 0 && a->right < 0) return kLevel;
