@@ -699,10 +699,13 @@ __device__ __forceinline__ int query_tiles(const Args& a, const Tile& t) {
   const int end = min(min(t.first + 127, t.n - 1) + (a.left < 0 ? kFar : a.left) + 1, t.n);
   return end > beg ? (end - beg + BK - 1) / BK : 0;
 }
-// A part's sums are 2 x 128 x D fp32 written and read again: 262 KB at D = 128, about as long as 4 steps of 64 queries.  Tiles of up to kWhole steps are left whole:
-// 16 sequences of 1 to 2048 (log), 32 / 8 heads of 128, causal, forward and backward: 505 / 496 / 579 us with 16 / 48 / 96.
-constexpr int kWhole = 48;
-__device__ __forceinline__ int split_of(int steps, int split) { return steps > kWhole ? split : 1; }
+// A part's sums are 2 x 128 x D fp32 written and read again: 131 KB at D = 128, about as long as 4 steps of 64 queries.  So a part has more than kPart steps:
+// 16 sequences of 1 to 2048 (log), 32 / 8 heads of 128, causal, forward and backward: 505 / 496 / 579 us with 8 / 24 / 48.
+constexpr int kPart = 24;
+__device__ __forceinline__ int split_of(int steps, int split) {  // (split: a power of two)
+  while (split > 1 && steps <= kPart * split) split >>= 1;
+  return split;
+}
 
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows.  The wave's
 // K and V fragments and its 128 accumulators stay in registers: 256 of them are just enough, and leave room for a second wave on the SIMD.  The second
@@ -912,7 +915,9 @@ __global__ __launch_bounds__(256) void attn_gqa_join_kernel(const Args a, const 
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.kv_heads, num = blockIdx.x / a.kv_heads, heads = a.heads / a.kv_heads;
   const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, num, order, lane);
-  if (tile.n == 0 || split_of(query_tiles(a, tile) * heads, split) == 1) return;
+  if (tile.n == 0) return;
+  const int parts = split_of(query_tiles(a, tile) * heads, split);
+  if (parts == 1) return;
   const f32x4* from = part + (size_t)blockIdx.x * split * (ND * 8 * 256) + tid;
   const int kj = tile.first + wid * 32 + (lane & 31);
   const long long row = tile.row0 + kj;
@@ -922,7 +927,7 @@ __global__ __launch_bounds__(256) void attn_gqa_join_kernel(const Args a, const 
 #pragma unroll
     for (int i = 0; i < ND * 4; ++i) {
       f32x4 sum = from[(which * ND * 4 + i) * 256];
-      for (int s = 1; s < split; ++s) sum += from[(s * ND * 8 + which * ND * 4 + i) * 256];
+      for (int s = 1; s < parts; ++s) sum += from[(s * ND * 8 + which * ND * 4 + i) * 256];
 #pragma unroll
       for (int e = 0; e < 4; ++e) g[i / 4][(i & 3) * 4 + e] = sum[e];
     }

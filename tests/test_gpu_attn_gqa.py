@@ -132,6 +132,8 @@ CASES += [
     ([1000, 1000, 1000], 2, 2, 128, True, (-1, -1), 0.2, 0, True),
     ([257] * 63 + [300], 1, 1, 16, True, (-1, -1), 0, 0, True),
     ([1900, 1], 8, 1, 32, True, (900, -1), 0, 0, True),
+    ([300], 64, 1, 64, False, (-1, -1), 0, 0, True),                 # the 64 query heads of one key head in up to 8 parts
+    ([700, 40], 32, 1, 128, True, (-1, -1), 0.1, 0, False),
 ]
 
 
@@ -222,6 +224,26 @@ def test_row_offsets_behind_two_gib():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     ga, gb = (ops.attn_gqa_bwd(*t, a[0], dctx, a[1], off, causal=True) for t in ((q, k, v), (sq, sk, sv)))
     assert all(torch.equal(x, y) for x, y in zip(ga, gb))
+
+
+def test_head_major_tensors_and_heads_that_share_their_memory():
+    """[heads, T, dim] tensors seen as [T, heads, dim], and keys and values whose heads (or rows) are one in memory"""
+    from cocodr_amd import ops
+    q, k, v, dctx, off = make([90, 230], 4, 2, 64, seed=15, fused=False)
+    turn = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    want = ops.attn_gqa_fwd(q, k, v, off, causal=True)
+    grads = ops.attn_gqa_bwd(q, k, v, want[0], dctx, want[1], off, causal=True)
+    ctx = turn(torch.empty_like(dctx))
+    got = ops.attn_gqa_fwd(turn(q), turn(k), turn(v), off, causal=True, out=ctx)
+    assert got[0] is ctx and torch.equal(ctx, want[0]) and torch.equal(got[1], want[1])
+    outs = tuple(turn(torch.empty(t.shape, dtype=torch.bfloat16, device="cuda")) for t in (q, k, v))
+    ops.attn_gqa_bwd(turn(q), turn(k), turn(v), ctx, turn(dctx), want[1], off, causal=True, out=outs)
+    assert all(torch.equal(x, y) for x, y in zip(outs, grads))
+    for one in (k[:, :1].expand(-1, 2, -1), k[:1].expand(320, -1, -1)):
+        a, b = (ops.attn_gqa_fwd(q, t, v, off, causal=True) for t in (one, one.contiguous()))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        ga, gb = (ops.attn_gqa_bwd(q, t, v, a[0], dctx, a[1], off, causal=True) for t in (one, one.contiguous()))
+        assert all(torch.equal(x, y) for x, y in zip(ga, gb))
 
 
 @pytest.mark.parametrize("stride", [7, 8, 1 << 24, 1 << 31])
