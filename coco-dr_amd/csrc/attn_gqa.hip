@@ -699,12 +699,13 @@ __device__ __forceinline__ int query_tiles(const Args& a, const Tile& t) {
   const int end = min(min(t.first + 127, t.n - 1) + (a.left < 0 ? kFar : a.left) + 1, t.n);
   return end > beg ? (end - beg + BK - 1) / BK : 0;
 }
-// A part's sums are 2 x 128 x D fp32 written and read again: 131 KB at D = 128, about as long as 4 steps of 64 queries.  So a part has more than kPart steps:
-// 16 sequences of 1 to 2048 (log), 32 / 8 heads of 128, causal, forward and backward: 505 / 496 / 579 us with 8 / 24 / 48.
-constexpr int kPart = 24;
-__device__ __forceinline__ int split_of(int steps, int split) {  // (split: a power of two)
-  while (split > 1 && steps <= kPart * split) split >>= 1;
-  return split;
+// In how many parts a tile's steps (tiles of 64 queries, of every head of the group) are summed: `split` is the most, a power of two, `part` the steps that
+// a part has to have more than.
+struct Split { int split, part; };
+__device__ __forceinline__ int parts_of(int steps, Split s) {
+  int n = s.split;
+  while (n > 1 && steps <= s.part * n) n >>= 1;
+  return n;
 }
 
 // dK, dV: 128 keys of one key head a workgroup, 32 a wave (lane = key), over the query heads of the group and tiles of 64 query rows.  The wave's
@@ -717,7 +718,7 @@ __device__ __forceinline__ int split_of(int steps, int split) {  // (split: a po
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, const uint16_t* __restrict__ dctx, const float* __restrict__ ndelta,
                                                               const float* __restrict__ nlse, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                                                              f32x4* __restrict__ part, int split, int order, int fill) {
+                                                              f32x4* __restrict__ part, Split split, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   if (fill) {
@@ -729,29 +730,34 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
         *reinterpret_cast<uint2*>(dv + row * a.dv_row + h * a.dv_head + tid * 4) = make_uint2(0u, 0u);
       }
   }
-  const int kvh = blockIdx.x % a.kv_heads, sub = blockIdx.x / a.kv_heads % split, num = blockIdx.x / (a.kv_heads * split);
+  const int kvh = blockIdx.x % a.kv_heads, sub = blockIdx.x / a.kv_heads % split.split, num = blockIdx.x / (a.kv_heads * split.split);
   const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, num, order, lane);
   if (tile.n == 0) return;
   const int n = tile.n, left = a.left < 0 ? kFar : a.left, right = a.right < 0 ? kFar : a.right;
   const int key0 = tile.first + wid * 32, kj = key0 + (lane & 31);
   const int last = min(tile.first + 127, n - 1), wlast = min(key0 + 31, n - 1);
   const int qbeg = max(tile.first - right, 0) & ~(BK - 1), qend = min(last + left + 1, n);
-  const int tiles = query_tiles(a, tile), heads = a.heads / a.kv_heads, G = heads / split_of(tiles * heads, split);  // (heads that this workgroup has)
-  if (sub * G >= heads) return;
-  f32x4* to = G < heads ? part + ((size_t)(num * a.kv_heads + kvh) * split + sub) * (DP / 4 * 256) : nullptr;  // where this part's sums go
+  const int tiles = query_tiles(a, tile), heads = a.heads / a.kv_heads, parts = parts_of(tiles * heads, split);
+  if (sub >= parts) return;
+  f32x4* to = parts > 1 ? part + ((size_t)(num * a.kv_heads + kvh) * split.split + sub) * (DP / 4 * 256) : nullptr;  // where this part's sums go
+  int from = 0, steps = tiles * heads;  // this part's first step, its steps
+  if (parts > 1) {
+    from = (int)((long long)steps * sub / parts);
+    steps = (int)((long long)steps * (sub + 1) / parts) - from;
+  }
+  const int h0 = kvh * heads + (parts > 1 ? from / tiles : 0), first = qbeg + (parts > 1 ? from % tiles * BK : 0);
   const float sl2 = a.scale * kLog2e;
   const bool alive = kj < n && (!a.mask || a.mask[tile.row0 + kj] != 0);
   const uint32_t live = (uint32_t)__ballot(alive);  // (both halves of the wave have the same 32 keys)
 
   constexpr int TB = BK * DP * 2, SB = 2 * TB + 2 * BK * 4, NC = DP / 16, ND = DP / 32;  // Q tile, dO tile, -lse and -delta of the rows
-  const int steps = tiles * G, h0 = kvh * heads + sub * G;
   const uint32_t lds0 = lds_addr(smem);
   Stager<DP> sq(a.q_row, a.dim, lane, wid), sd(a.do_row, a.dim, lane, wid);
   // the tile that is sent for next: its first row, where its Q, dO and statistics are, and from there to the next head's first tile
-  int fq = qbeg;
-  const uint16_t* qs = a.q + (long long)(tile.row0 + qbeg) * a.q_row + h0 * a.q_head;
-  const uint16_t* ds = dctx + (long long)(tile.row0 + qbeg) * a.do_row + h0 * a.do_head;
-  const float* st = (wid == 0 ? nlse : ndelta) + (size_t)h0 * a.T + tile.row0 + qbeg;
+  int fq = first;
+  const uint16_t* qs = a.q + (long long)(tile.row0 + first) * a.q_row + h0 * a.q_head;
+  const uint16_t* ds = dctx + (long long)(tile.row0 + first) * a.do_row + h0 * a.do_head;
+  const float* st = (wid == 0 ? nlse : ndelta) + (size_t)h0 * a.T + tile.row0 + first;
   const long long qwrap = a.q_head - (long long)tiles * BK * a.q_row, dwrap = a.do_head - (long long)tiles * BK * a.do_row;
   const int swrap = a.T - tiles * BK;
   auto fetch = [&](uint32_t to) {
@@ -795,7 +801,7 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
     for (int r = 0; r < 16; ++r) { gk[dt][r] = 0.f; gv[dt][r] = 0.f; }
   Bits<DP> f(lds0, lane);
 
-  int q0 = qbeg, left_ = steps;  // the tile that is worked on, the tiles that are left
+  int q0 = first, left_ = steps;  // the tile that is worked on, the tiles that are left
   auto work = [&](auto buf_) {
     constexpr int QA = decltype(buf_)::value * SB, DA = QA + TB;
     dma_wait();
@@ -910,15 +916,15 @@ __global__ __launch_bounds__(256, 2) void attn_gqa_dkv_kernel(const Args a, cons
 // The sums of the parts, in their order.  A thread has the accumulators that the same thread of the parts' workgroups left.
 template <int DP>
 __global__ __launch_bounds__(256) void attn_gqa_join_kernel(const Args a, const f32x4* __restrict__ part, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                                                            int split, int order) {
+                                                            Split split, int order) {
   constexpr int ND = DP / 32;
   const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.kv_heads, num = blockIdx.x / a.kv_heads, heads = a.heads / a.kv_heads;
   const Tile tile = find_tile<128>(a.seq_off, a.B, a.T, num, order, lane);
   if (tile.n == 0) return;
-  const int parts = split_of(query_tiles(a, tile) * heads, split);
+  const int parts = parts_of(query_tiles(a, tile) * heads, split);
   if (parts == 1) return;
-  const f32x4* from = part + (size_t)blockIdx.x * split * (ND * 8 * 256) + tid;
+  const f32x4* from = part + (size_t)blockIdx.x * split.split * (ND * 8 * 256) + tid;
   const int kj = tile.first + wid * 32 + (lane & 31);
   const long long row = tile.row0 + kj;
 #pragma unroll
@@ -972,14 +978,17 @@ Order order_of(const Args* a, bool keys) {
   return (a->right >= 0) != keys ? kUp : kDown;
 }
 
-// Tiles of the dK / dV kernel, and in how many parts it sums the heads of a group.  The chip holds 512 of its workgroups: with fewer tiles than that the
-// longest one, 4 x 2048 rows of queries at 2.9 us a step of 64 in the case above, is all that runs in the end (373 us of 600).  Two parts there: 232 and
-// 19 us for the join; four, 1888 workgroups: slower again (543 us for all against 496).
+// Tiles of the dK / dV kernel, and in how many parts it sums a tile's steps.  The chip holds 512 of its workgroups: with fewer tiles than that the
+// longest one is all that runs in the end - 16 sequences of 1 to 2048, causal, 32 / 8 heads of 128: 4 x 2048 rows of queries at 2.9 us a step of 64, 373 us of 600.
+// As many parts as fit the chip twice (there: two, 205 us and 20 for the join; four, 1888 workgroups, took 543 us for all against 496), and each of more
+// steps than what its sums cost, 2 x 128 x D fp32 written and read again.  Backward, us, with parts of more than 48 / 24 / 12 / 8 steps:
+//   heads of 128, 32 / 8, causal: 2048 rows 290 / 235 / 191 / 191 (whole: 338), 3 x 2048 440 / 427 / 405 / 394; the 16 sequences with the forward 444 / 448 / 451
+//   from 24 on; heads of 64, whose steps are half as long: 4 x 512, 12 heads 34 / 34 / 42 / 37, sequences of 1000, 200 and 50, 16 heads 51 / 51 / 52 / 54
 long long units_of(const Args* a) { return ((long long)a->T / 128 + a->B) * a->kv_heads; }
-int split_for(const Args* a) {
-  const int G = a->heads / a->kv_heads;
-  int s = 1;
-  while (G % (2 * s) == 0 && units_of(a) * 2 * s <= 1024) s *= 2;
+Split split_for(const Args* a) {
+  Split s{1, a->dim <= 64 ? 24 : 12};
+  const long long steps = ((long long)a->T / 64 + 1) * (a->heads / a->kv_heads);  // of the longest tile, at most
+  while (units_of(a) * 2 * s.split <= 1024 && steps > (long long)s.part * 2 * s.split) s.split *= 2;
   return s;
 }
 size_t stats_floats(const Args* a) { return ((size_t)2 * a->T * a->heads + 3) & ~(size_t)3; }  // (what is behind them starts at a multiple of 16 bytes)
@@ -1022,8 +1031,8 @@ extern "C" int cocodr_attn_gqa_fwd(const cocodr_attn_gqa_args* args, uint16_t* c
 
 extern "C" size_t cocodr_attn_gqa_bwd_workspace_floats(const cocodr_attn_gqa_args* a) {
   if (!a || a->T <= 0 || a->B <= 0 || a->kv_heads <= 0 || a->heads < a->kv_heads) return 0;
-  const int split = split_for(a);
-  return stats_floats(a) + (split > 1 ? (size_t)units_of(a) * split * part_floats(a) : 0);
+  const Split s = split_for(a);
+  return stats_floats(a) + (s.split > 1 ? (size_t)units_of(a) * s.split * part_floats(a) : 0);
 }
 
 extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* args, const uint16_t* ctx, const uint16_t* dctx, const float* lse, uint16_t* dq,
@@ -1045,17 +1054,17 @@ extern "C" int cocodr_attn_gqa_bwd(const cocodr_attn_gqa_args* args, const uint1
   hipStream_t st = (hipStream_t)stream;
   float *ndelta = workspace, *nlse = workspace + (size_t)a->T * a->heads;
   f32x4* part = reinterpret_cast<f32x4*>(workspace + stats_floats(a));
-  const int split = split_for(a);
+  const Split split = split_for(a);
   const Order rows = order_of(a, false), keys = order_of(a, true);
-  const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)(units_of(a) * split)), gj((unsigned)units_of(a));
+  const dim3 gq((unsigned)((a->T / 128 + a->B) * a->heads)), gk((unsigned)(units_of(a) * split.split)), gj((unsigned)units_of(a));
   if (a->dim <= 64) {
     hipLaunchKernelGGL(attn_gqa_dq_kernel<64>, gq, dim3(256), kv_lds(64), st, *a, ctx, dctx, lse, ndelta, nlse, dq, rows, fill);
     hipLaunchKernelGGL(attn_gqa_dkv_kernel<64>, gk, dim3(256), qd_lds(64), st, *a, dctx, ndelta, nlse, dk, dv, part, split, keys, fill);
-    if (split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<64>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
+    if (split.split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<64>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
   } else {
     hipLaunchKernelGGL(attn_gqa_dq_kernel<128>, gq, dim3(256), kv_lds(128), st, *a, ctx, dctx, lse, ndelta, nlse, dq, rows, fill);
     hipLaunchKernelGGL(attn_gqa_dkv_kernel<128>, gk, dim3(256), qd_lds(128), st, *a, dctx, ndelta, nlse, dk, dv, part, split, keys, fill);
-    if (split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<128>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
+    if (split.split > 1) hipLaunchKernelGGL(attn_gqa_join_kernel<128>, gj, dim3(256), 0, st, *a, part, dk, dv, split, keys);
   }
   CK_LAUNCH("attn_gqa_bwd");
   return COCODR_OK;

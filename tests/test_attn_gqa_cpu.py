@@ -46,8 +46,10 @@ def test_outputs_that_overlap_or_are_missing(lib):  # noqa: F811
     need = lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(a))
     assert need >= 2 * 100 * 8
     assert bwd(ws=4104) == -1 and b"workspace" in lib.cocodr_last_error()
-    # few tiles of a group of query heads: room for the parts of dk and dv, 2 x 128 x 64 floats a tile and part
-    assert lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(args(heads=16))) >= 2 * 100 * 16 + 2 * (100 // 128 + 3) * 4 * 2 * 128 * 64
+    # few tiles with many steps: room for the parts of dk and dv, 2 x 128 x 64 floats a tile and part; none for short ones
+    a = args(T=4096, B=3, heads=32, kv_heads=8)
+    assert lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(a)) >= 2 * 4096 * 32 + 2 * (4096 // 128 + 3) * 8 * 2 * 128 * 64
+    assert lib.cocodr_attn_gqa_bwd_workspace_floats(C.byref(args(T=32, B=1))) == 2 * 32 * 8
     assert bwd(floats=need - 1) == -3 and b"workspace" in lib.cocodr_last_error() and bwd(ws=0) == -3
 
 

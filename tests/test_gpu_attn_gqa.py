@@ -133,6 +133,8 @@ CASES += [
     ([257] * 63 + [300], 1, 1, 16, True, (-1, -1), 0, 0, True),
     ([1900, 1], 8, 1, 32, True, (900, -1), 0, 0, True),
     ([300], 64, 1, 64, False, (-1, -1), 0, 0, True),                 # the 64 query heads of one key head in up to 8 parts
+    ([2100], 1, 1, 128, False, (-1, -1), 0.1, 5, True),              # one head's 33 tiles of queries in two parts
+    ([1500, 90], 6, 2, 72, True, (-1, -1), 0, 0, True),              # three heads: parts begin inside a head
     ([700, 40], 32, 1, 128, True, (-1, -1), 0.1, 0, False),
 ]
 
