@@ -134,6 +134,9 @@ CASES += [
     ([1900, 1], 8, 1, 32, True, (900, -1), 0, 0, True),
     ([300], 64, 1, 64, False, (-1, -1), 0, 0, True),                 # the 64 query heads of one key head in up to 8 parts
     ([2100], 1, 1, 128, False, (-1, -1), 0.1, 5, True),              # one head's 33 tiles of queries in two parts
+    ([2500], 2, 1, 64, True, (-1, -1), 0.3, 0, True),
+    ([1800, 60], 1, 1, 80, False, (1500, 300), 0, 9, False),
+    ([3, 2200], 2, 2, 32, False, (-1, 700), 0.6, 0, True),
     ([1500, 90], 6, 2, 72, True, (-1, -1), 0, 0, True),              # three heads: parts begin inside a head
     ([700, 40], 32, 1, 128, True, (-1, -1), 0.1, 0, False),
 ]
