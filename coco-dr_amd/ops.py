@@ -214,9 +214,9 @@ def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
 def _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale) -> N.AttnGqaArgs:
     _rows3(q, "q")
     T, heads, dim = q.shape
-    _rows3(k, "k")
-    kv_heads = k.shape[1]
-    _rows3(k, "k", (T, kv_heads, dim))
+    kv_heads = _rows3(k, "k").shape[1]
+    if k.shape[0] != T or k.shape[2] != dim:
+        raise ValueError(f"k: expected shape {(T, kv_heads, dim)}, got {tuple(k.shape)}")
     _rows3(v, "v", (T, kv_heads, dim))
     _req(seq_off, I32, "seq_off", 1)
     if T < 1 or seq_off.shape[0] < 2:
@@ -249,8 +249,8 @@ def attn_gqa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: tor
     anything; the others have to be finite.  ``out`` shares no memory with q, k and v."""
     a = _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale)
     with _on_device(q, k, v, seq_off, mask, out):
-        ctx = torch.empty(q.shape, dtype=BF16, device=q.device) if out is None else _rows3(out, "out", tuple(q.shape))
-        lse = torch.empty((a.heads, a.T), dtype=F32, device=q.device)
+        ctx = q.new_empty((a.T, a.heads, a.dim)) if out is None else _rows3(out, "out", tuple(q.shape))
+        lse = q.new_empty((a.heads, a.T), dtype=F32)
         a.o_row, a.o_head, _ = ctx.stride()
         check(lib().cocodr_attn_gqa_fwd(C.byref(a), _addr(ctx), _addr(lse), int(out is None), _stream(q)), "attn_gqa_fwd")
     return ctx, lse
@@ -270,13 +270,13 @@ def attn_gqa_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: torch.T
         raise ValueError("attn_gqa_bwd: out holds dq, dk and dv")
     with _on_device(q, k, v, seq_off, mask, ctx, dctx, lse, *(out or ())):
         if out is None:
-            dq, dk, dv = (torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
+            dq, dk, dv = (t.new_empty(tuple(t.shape)) for t in (q, k, v))
         else:
             dq, dk, dv = (_rows3(t, n, tuple(x.shape)) for t, n, x in zip(out, ("dq", "dk", "dv"), (q, k, v)))
         (a.o_row, a.o_head, _), (a.do_row, a.do_head, _) = ctx.stride(), dctx.stride()
         (a.dq_row, a.dq_head, _), (a.dk_row, a.dk_head, _), (a.dv_row, a.dv_head, _) = dq.stride(), dk.stride(), dv.stride()
         floats = lib().cocodr_attn_gqa_bwd_workspace_floats(C.byref(a))
-        ws = torch.empty(floats, dtype=F32, device=q.device)
+        ws = q.new_empty((floats,), dtype=F32)
         check(lib().cocodr_attn_gqa_bwd(C.byref(a), _addr(ctx), _addr(dctx), _addr(lse), _addr(dq), _addr(dk), _addr(dv), int(out is None), _addr(ws), floats,
                                         _stream(q)), "attn_gqa_bwd")
     return dq, dk, dv
@@ -297,7 +297,7 @@ def embed_fwd(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out
         raise ValueError(f"embed_fwd: out_dtype {out_dtype}: {F32} or {BF16} is wanted")
     V, H = table.shape
     with _on_device(table, ids):
-        out = torch.empty(tuple(ids.shape) + (H,), dtype=out_dtype, device=table.device)
+        out = table.new_empty(tuple(ids.shape) + (H,), dtype=out_dtype)
         check(lib().cocodr_embed_fwd(_addr(ids), int(ids.dtype == I64), _addr(table), int(table.dtype == F32), _addr(out), int(out_dtype == F32),
                                      ids.numel(), H, V, float(scale), _stream(table)), "embed_fwd")
     return out

@@ -321,6 +321,10 @@ def test_refusals_on_the_device():
         ops.attn_gqa_fwd(q.half(), k, v, off)
     with pytest.raises(ValueError, match="shape"):
         ops.attn_gqa_fwd(q, k, v[:32], off)
+    with pytest.raises(ValueError, match="k: expected shape"):
+        ops.attn_gqa_fwd(q, k[:63], v[:63], off)
+    with pytest.raises(ValueError, match="k: expected shape"):
+        ops.attn_gqa_fwd(q, k[:, :, :32], v, off)
     with pytest.raises(ValueError, match="adjacent"):
         ops.attn_gqa_fwd(q, k.transpose(1, 2).contiguous().transpose(1, 2), v, off)
     with pytest.raises(ValueError, match="16-byte"):
