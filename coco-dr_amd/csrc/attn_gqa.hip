@@ -11,7 +11,6 @@
 // lane ^ 32) and straight where it holds a key (dK, dV); in both the fp32 accumulators, rounded to bf16, are the next product's B
 // operand as they stand, and that product's A operand is read from LDS with the transposing read in the same row order.
 // bf16 is what the matrix pipe takes: P and dS are rounded to it (half a step, at most 2^-8 of each element); every sum is fp32.
-#include <limits.h>
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -943,6 +942,7 @@ __global__ __launch_bounds__(256) void attn_gqa_join_kernel(const Args a, const 
 }
 
 // ------------------------------------------------------------------------------------------------ host
+constexpr long long kMaxGroups = (1ll << 24) - 1;  // workgroups of 256: a launch counts its work-items in 32 bits
 constexpr long long kMaxStride = 1ll << 23;  // elements: 64 rows of it stay inside a buffer descriptor's 31-bit offsets
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -965,7 +965,7 @@ int check(const Args* a, const char* what) {
   CK_ARG(aligned16(a->q) && aligned16(a->k) && aligned16(a->v), "%s: q, k, v must be 16-byte aligned", what);
   CK_ARG(stride_ok(a->q_row, a->q_head, a->T, a->heads) && stride_ok(a->k_row, a->k_head, a->T, a->kv_heads) && stride_ok(a->v_row, a->v_head, a->T, a->kv_heads), "%s: strides must be multiples of 8 elements, rows less than 2^23 apart", what);
   const long long units = ((long long)a->T / 128 + a->B) * a->heads;
-  CK_ARG(units <= INT_MAX, "%s: too many rows and heads for one launch", what);
+  CK_ARG(units <= kMaxGroups, "%s: %d rows in %d sequences of %d heads are too many for one launch (rows / 128 + sequences, times heads: below 2^24)", what, a->T, a->B, a->heads);
   return COCODR_OK;
 }
 

@@ -185,7 +185,8 @@ int cocodr_attn_bwd_drop(const uint16_t* qkv, const int32_t* mask, const uint16_
  * Backward: recomputes the probabilities from q, k and lse; dk and dv sum over the query heads of a key head's group.  No atomics:
  * the same inputs give the same bits.  workspace: cocodr_attn_gqa_bwd_workspace_floats(args) floats, 16-byte aligned.
  * Requirements: dim % 8 == 0, dim <= 128; pointers (not lse, seq_off, mask) 16-byte aligned; strides multiples of 8, rows less than
- * 2^23 elements apart; rows and heads of an output do not overlap, and no output shares memory with an input; scale > 0; T < 2^30.
+ * 2^23 elements apart; rows and heads of an output do not overlap, and no output shares memory with an input; scale > 0; T < 2^30;
+ * (T / 128 + B) * heads < 2^24 (the workgroups of a launch).
  * ------------------------------------------------------------------------------------------ */
 typedef struct {
   const uint16_t *q, *k, *v;
