@@ -207,6 +207,13 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def _int32(what: str, *values: int) -> None:
+    """the C interface takes these as 32-bit numbers, and ctypes cuts a longer one without a word"""
+    for v in values:
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise ValueError(f"{what}: {v} does not fit 32 bits")
+
+
 def _addr(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -230,6 +237,7 @@ def _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale) -> N.AttnGqaAr
         if right > 0:
             raise ValueError(f"attn_gqa: causal rows see nothing to their right (window {tuple(window)})")
         right = 0
+    _int32("attn_gqa", T, heads, kv_heads, dim, seq_off.shape[0], left, right)
     scale = dim ** -0.5 if scale is None else float(scale)
     (q0, q1, _), (k0, k1, _), (v0, v1, _) = q.stride(), k.stride(), v.stride()
     return N.AttnGqaArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), seq_off.data_ptr(), _addr(mask), q0, q1, k0, k1, v0, v1,
@@ -296,6 +304,7 @@ def embed_fwd(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out
     if out_dtype not in (F32, BF16):
         raise ValueError(f"embed_fwd: out_dtype {out_dtype}: {F32} or {BF16} is wanted")
     V, H = table.shape
+    _int32("embed_fwd", ids.numel(), V, H)
     with _on_device(table, ids):
         out = table.new_empty(tuple(ids.shape) + (H,), dtype=out_dtype)
         check(lib().cocodr_embed_fwd(_addr(ids), int(ids.dtype == I64), _addr(table), int(table.dtype == F32), _addr(out), int(out_dtype == F32),
@@ -312,6 +321,7 @@ def embed_bwd(dout: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float
     if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"embed_bwd: dout {tuple(dout.shape)} is not ids {tuple(ids.shape)} + [H]")
     H, V = dout.shape[-1], int(vocab)
+    _int32("embed_bwd", ids.numel(), V, H)
     if accumulate and out is None:
         raise ValueError("embed_bwd: accumulate needs the tensor to add to (out)")
     if out is not None:
