@@ -29,6 +29,7 @@ constexpr int kMap = 1 << 16;     // positions that the bitmap holds at a time (
 constexpr int kBatch = 1024;      // ordered positions at a time
 constexpr int kWide = 512;        // columns of a wave: 64 lanes x 8
 constexpr int kLeast = 8;         // lanes of the narrowest slice: 64 columns, 32 rows at a time
+constexpr int kGroups = 1 << 23;  // workgroups of a lookup: 256 work-items each, fewer than 2^32 in all
 
 struct Ids {
   const void* p;
@@ -378,7 +379,8 @@ extern "C" int cocodr_embed_fwd(const void* ids, int ids_i64, const void* table,
   if (n == 0) return COCODR_OK;
   if (int rc = check("embed_fwd", ids, table, out, n, H, vocab, scale)) return rc;
   hipStream_t st = (hipStream_t)stream;
-  const int per = std::max(1, 2048 / (H / 4));
+  // (2048 lanes' work a workgroup; more where a launch, which counts its work-items in 32 bits, could not have that many)
+  const int per = std::max(std::max(1, 2048 / (H / 4)), (n + kGroups - 1) / kGroups);
   const dim3 grid((unsigned)((n + per - 1) / per));
   const Ids d{ids, ids_i64};
   if (table_f32) {

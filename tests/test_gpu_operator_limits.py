@@ -31,3 +31,22 @@ def test_a_vocabulary_that_32_bits_cannot_hold(vocab):
     from cocodr_amd import ops
     with pytest.raises(ValueError, match="32 bits"):
         ops.embed_bwd(torch.ones((3, 8), device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), vocab)
+
+
+def test_a_lookup_of_more_rows_than_a_launch_has_workgroups():
+    """2^24 rows of 4104 columns, of which a workgroup would take one: 138 GB of results"""
+    from cocodr_amd import ops
+    n, H = (1 << 24) + 3, 4104
+    if torch.cuda.mem_get_info()[0] < n * H * 2 + (1 << 33):
+        pytest.skip("needs 146 GB of free device memory")
+    table = torch.arange(5 * H, device="cuda").remainder(251).view(5, H).to(torch.bfloat16)
+    ids = torch.arange(n, device="cuda", dtype=torch.int32).remainder(7)  # (5 and 6: padding)
+    got = ops.embed_fwd(ids, table)
+    for a in (0, 1 << 23, (1 << 24) - 2000, n - 2000):
+        part = ids[a:a + 2000].long()
+        want = torch.where((part < 5)[:, None], table[part.clamp(max=4)], torch.zeros((), dtype=torch.bfloat16, device="cuda"))
+        assert torch.equal(got[a:a + 2000], want), a
+    for col in (0, 2051, H - 1):  # every row
+        assert torch.equal(got[:, col].float(), torch.where(ids < 5, table[ids.clamp(max=4).long(), col].float(), 0.0))
+    del got
+    torch.cuda.empty_cache()
