@@ -3,8 +3,8 @@
 // An id outside [0, vocab) is a padding row: zeros out, no gradient.  Both are bound by memory: the looked-up rows in and out; dout in and
 // the dense gradient (the whole table, zeros included) out.
 //
-// The gradient adds no floats atomically: its sums run in the order of the tokens, so the same inputs give the same bits.  The tokens of each id are
-// brought together by counting:
+// The gradient adds no floats atomically, so the same inputs give the same bits: an id of up to kFew tokens is added up in their order, one with more
+// in a fixed tree that follows from their number and positions and, above kMany, from n.  The tokens of each id are brought together by counting:
 //   rank    a token's number among those of its id, and how many there are (integer atomics: their order is arbitrary)
 //   alloc   every id that occurs takes a stretch of the position list and goes, by the number of its tokens, to the rows that waves work on (up to
 //           kFew), to the tasks of whole workgroups (up to kMany) or to the list of those that several workgroups share

@@ -314,9 +314,9 @@ def embed_fwd(ids: torch.Tensor, table: torch.Tensor, *, scale: float = 1.0, out
 
 def embed_bwd(dout: torch.Tensor, ids: torch.Tensor, vocab: int, *, scale: float = 1.0, out: Optional[torch.Tensor] = None,
               accumulate: bool = False) -> torch.Tensor:
-    """The gradient [vocab, H] fp32 of embed_fwd's table: scale * the sum of dout's rows (bf16 or fp32, ids.shape + [H]) of each id, summed
-    in the order of the tokens (deterministic: no float atomics); zero rows for ids that do not occur.  ``out`` receives it; with
-    ``accumulate`` it is added to what ``out`` holds (rows of other ids are not touched)."""
+    """The gradient [vocab, H] fp32 of embed_fwd's table: scale * the sum of dout's rows (bf16 or fp32, ids.shape + [H]) of each id, the same bits
+    for the same inputs (no float atomics; up to 16 tokens of an id in their order, more in a fixed tree); zero rows for ids that do not
+    occur.  ``out`` receives it; with ``accumulate`` it is added to what ``out`` holds (rows of other ids are not touched)."""
     _req_any(dout, (F32, BF16), "dout"); _req_any(ids, (I32, I64), "ids")
     if dout.dim() != ids.dim() + 1 or tuple(dout.shape[:-1]) != tuple(ids.shape):
         raise ValueError(f"embed_bwd: dout {tuple(dout.shape)} is not ids {tuple(ids.shape)} + [H]")

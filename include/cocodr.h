@@ -271,9 +271,10 @@ int cocodr_scatter_cls_grad(const float* dE, uint16_t* d_last, int B, int L, int
 /* Embedding lookup with scaling: out[t] = scale * table[ids[t]] (rows of H; bf16 or fp32 each, *_f32 != 0: fp32), and its gradient
  * dtable[v] = scale * sum over ids[t] == v of dout[t] (fp32 [vocab, H], all rows written; accumulate != 0: added to what is there), e.g.
  * the token embedding of a decoder backbone, scaled by sqrt(H) in some.  ids int32 or int64 (ids_i64 != 0) [n]; an id outside
- * [0, vocab) is padding: a zero row, no gradient.  The gradient's sums run in the order of the tokens, without float atomics: the same
- * inputs give the same bits.  H % 8 == 0; tensors 16-byte aligned; workspace: cocodr_embed_bwd_workspace_bytes(n, H, vocab) bytes,
- * 16-byte aligned. */
+ * [0, vocab) is padding: a zero row, no gradient.  The gradient adds no floats atomically: the same inputs give the same bits.  Up to 16
+ * tokens of an id are added one after the other in the order of the tokens; more in a fixed tree that follows from their number, their
+ * positions and, above 8192 of them, n.  H % 8 == 0; tensors 16-byte aligned; workspace: cocodr_embed_bwd_workspace_bytes(n, H, vocab)
+ * bytes, 16-byte aligned. */
 int cocodr_embed_fwd(const void* ids, int ids_i64, const void* table, int table_f32, void* out, int out_f32, int n, int H, int vocab,
                      float scale, cocodr_stream_t stream);
 size_t cocodr_embed_bwd_workspace_bytes(int n, int H, int vocab);
