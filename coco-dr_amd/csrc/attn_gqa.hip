@@ -21,9 +21,11 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kLow = -1e30f;  // where a running maximum starts: finite, so that a row without any key gives exp2(-inf - kLow) = 0 and no NaN
+// Where a running maximum starts: finite, so that a row without any key gives exp2(-inf - kLow) = 0 and no NaN, and far below every score that fp32
+// can subtract from another (up to 2^24 or so; a row of scores below kLow would pass for one without keys).
+constexpr float kLow = -1e30f;
 // A running maximum that is outgrown by less than 2^kGrow is left as it is: terms of up to 2^kGrow are as exact in fp32 and bf16 as those below 1, and
-// the accumulators, at most 2^kGrow times a sum of |v|, stay finite.
+// the accumulators are at most 2^kGrow times a sum of |v|: finite below 2^108.
 constexpr float kGrow = 20.0f;
 constexpr int kFar = 1 << 30;   // an unlimited window; i + kFar stays inside an int for every row index < 2^30
 constexpr int BK = 64;          // rows of a staged tile

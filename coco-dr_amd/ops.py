@@ -254,7 +254,7 @@ def attn_gqa_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, seq_off: tor
     the key is not seen; window (left, right) = how many rows before and behind its own a query sees (-1: all); scale: 1 / sqrt(dim)
     unless given.  A row that sees nothing gets ctx 0 and lse -inf, and so do the rows of no sequence - unless ``out`` is given: there
     they are left as they are (their lse is unspecified).  Rows of k and v that the mask excludes, or that belong to no sequence, may hold
-    anything; the others have to be finite.  ``out`` shares no memory with q, k and v."""
+    anything; the others have to be finite, and so has q; scores up to 2^24 in magnitude.  ``out`` shares no memory with q, k and v."""
     a = _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale)
     with _on_device(q, k, v, seq_off, mask, out):
         ctx = q.new_empty((a.T, a.heads, a.dim)) if out is None else _rows3(out, "out", tuple(q.shape))
@@ -269,7 +269,8 @@ def attn_gqa_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, ctx: torch.T
                  scale: Optional[float] = None, out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None):
     """(dq [T, heads, dim], dk, dv [T, kv_heads, dim]) bf16 of attn_gqa_fwd with the same q .. scale, its ctx and lse, and the gradient
     dctx of ctx (ctx and dctx with any strides as q's; they need not be the same).  The rows of no sequence get zeros; with ``out`` (three
-    tensors to write to, e.g. views of one fused gradient; no memory in common with the inputs) they are left as they are.  Deterministic."""
+    tensors to write to, e.g. views of one fused gradient; no memory in common with the inputs or one another) they are left as they are.
+    dctx has to be finite in every row of a sequence.  Deterministic."""
     a = _attn_gqa_args(q, k, v, seq_off, causal, window, mask, scale)
     _rows3(ctx, "ctx", tuple(q.shape)); _rows3(dctx, "dctx", tuple(q.shape)); _req(lse, F32, "lse", 2)
     if tuple(lse.shape) != (a.heads, a.T):

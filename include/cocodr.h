@@ -180,12 +180,15 @@ int cocodr_attn_bwd_drop(const uint16_t* qkv, const int32_t* mask, const uint16_
  *   ctx_i = sum_j softmax_j(scale q_i . k_j) v_j [T, heads, dim] bf16, lse [heads, T] fp32 = log sum_j exp(scale q_i . k_j);
  *   a row that sees nothing gets ctx = 0, lse = -inf and zero gradients.  K and V rows behind a sequence or masked out are not read
  *   (they may hold anything, NaN too); keys that a row does not see because of causality or its window count as 0 times their values, so
- *   the others have to be finite.
+ *   the others have to be finite, and so have q and dctx in every row of a sequence, also in one that sees nothing.
+ *   Range: scores of magnitude up to 2^24, where fp32 still tells 1 from 2, and keys whose |v| add up to less than 2^108 (terms up to 2^20
+ *   times that of the running maximum are added before the division).  The backward's probabilities come from lse in fp32: off by
+ *   up to |lse| 2^-22 of themselves.
  * fill: rows that belong to no sequence get ctx = 0 and lse = -inf, zero gradients (1), or are left as they are (0).
  * Backward: recomputes the probabilities from q, k and lse; dk and dv sum over the query heads of a key head's group.  No atomics:
  * the same inputs give the same bits.  workspace: cocodr_attn_gqa_bwd_workspace_floats(args) floats, 16-byte aligned.
  * Requirements: dim % 8 == 0, dim <= 128; pointers (not lse, seq_off, mask) 16-byte aligned; strides multiples of 8, rows less than
- * 2^23 elements apart; rows and heads of an output do not overlap, and no output shares memory with an input; scale > 0; T < 2^30;
+ * 2^23 elements apart; rows and heads of an output do not overlap, and no output shares memory with an input or another output; scale > 0; T < 2^30;
  * (T / 128 + B) * heads < 2^24 (the workgroups of a launch).
  * ------------------------------------------------------------------------------------------ */
 typedef struct {

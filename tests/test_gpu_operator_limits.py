@@ -50,3 +50,22 @@ def test_a_lookup_of_more_rows_than_a_launch_has_workgroups():
         assert torch.equal(got[:, col].float(), torch.where(ids < 5, table[ids.clamp(max=4).long(), col].float(), 0.0))
     del got
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_at_the_end_of_their_range(D, sign):
+    """all of a row's scores 2^24 or -2^24: each key counts the same, ctx is the mean of v.  Equal scores give equal probabilities, at most 2 times too
+    large or small all together (half of 2^24's step): what is left are the roundings of P and ctx, 2^-8 each, and n 2^-24 of the sums.
+    lse is the score + log n = 5.3, off by at most 0.7 where log2 of the sum is added (half of the step at 2^24.5), 1.5 by scale log2 e, 0.5 by ln 2 and 1
+    at the end: below 10 in all.  Values near 2^92 do not overflow on the way"""
+    from cocodr_amd import ops
+    n, H = 200, 2
+    q = torch.full((n, H, D), 2.0 ** 9, dtype=torch.bfloat16, device="cuda")
+    k = torch.full((n, 1, D), sign * 2.0 ** 9, dtype=torch.bfloat16, device="cuda")
+    v = (torch.rand((n, 1, D), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda") * 2.0 ** 92).to(torch.bfloat16)
+    off = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    ctx, lse = ops.attn_gqa_fwd(q, k, v, off, scale=64.0 / D)
+    assert ((lse.double() - sign * 2.0 ** 24).abs() <= 10).all()
+    want = v.double().mean(0, keepdim=True).expand(n, H, D)
+    assert ((ctx.double() - want).abs() <= want * (2 * 2.0 ** -8 + 2.0 ** -14)).all()
