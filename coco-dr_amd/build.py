@@ -39,6 +39,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".h", ".inc"))]
     headers.append(os.path.join(os.path.dirname(HERE), "include", "cocodr.h"))
+    headers.append(os.path.abspath(__file__))  # the flags stand here
     jobs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
