@@ -182,7 +182,7 @@ template <int DP> __device__ __forceinline__ void store_T(uint16_t* row, const f
 // The tiles of TILE rows are numbered without a table, and a launch has T / TILE + B workgroups, at least as many as there are tiles.
 //   up to 256 sequences: consecutive numbers in the order of the rows, from a sum over the sequences that every wave makes, four a lane; the numbers
 //     that no tile has come last, where they hold nobody up (64 x 128 rows, 12 heads, forward and backward: 58 us; 75 with the numbers below, every
-//     second of which is empty there)
+//     second of which is empty there; forward of 256 sequences of 20 to 256, 16 heads, 70 us, of 257 with the numbers below 75, of 512 145)
 //   more: tile t of sequence b has the number off[b] / TILE + b + t - rounding down and the + b leave a sequence at least as many numbers as it has
 //     tiles -, and number -> sequence is the last b with off[b] / TILE + b <= number: a search 64 wide
 // When sequences are long and few, the numbers go by the work of a tile instead, the most first: a workgroup with much to do that starts
@@ -379,12 +379,12 @@ __device__ __forceinline__ void fill_gaps(const Args& a, uint16_t* ctx, float* l
 
 // A workgroup has 128 query rows of one head, each of its four waves 32 of them; K and V pass through LDS in tiles of 64 keys, two tiles each, so that
 // a tile is on its way while the one before is worked on.  Scores, statistics and the output never leave the registers: one pass over the keys.
-// Heads of 128, long sequences: bound by the matrix pipe, and that by power: 8192 causal, 32 / 8 heads, 570 us = 965 TFLOP/s, where the pipe is 48 % busy
+// Heads of 128, long sequences: bound by the matrix pipe, and that by power: 8192 causal, 32 / 8 heads, 566 us = 971 TFLOP/s, where the pipe is 48 % busy
 // at 1.9 GHz; 64 rows a wave (one wave a SIMD, half the LDS traffic) took 580 us at 2.4 GHz, eight waves sharing a tile 571.  So 32 rows and two
 // workgroups a CU, which short sequences want too (129 against 84 us with eight waves, 256 sequences of 20 to 256).
 // Heads of 64, short sequences: bound by what stands before the first product - offsets, mask, first tile, each waiting for the one before, 5 of a
 // workgroup's 10 us - so as many workgroups at once as registers allow (122: four a CU; addresses by flipped bits instead of a register each): 256
-// sequences of 20 to 256, 16 heads, masked: 71 us, 2.7 TB/s.  Two heads after one another in a workgroup saved nothing (71 - 75 us).
+// sequences of 20 to 256, 16 heads, masked: 70 us, 2.8 TB/s.  Two heads after one another in a workgroup saved nothing (71 - 75 us).
 template <int DP>
 __global__ __launch_bounds__(256, DP == 64 ? 4 : 2) void attn_gqa_fwd_kernel(const Args a, uint16_t* __restrict__ ctx, float* __restrict__ lse, int order, int fill) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -519,8 +519,10 @@ __device__ __forceinline__ int keys_of(int i, int n, int left, int right) { retu
 // dQ: 128 query rows of one head a workgroup, 32 a wave (lane = query), over tiles of 64 keys as in the forward.  A wave has its rows of dO in
 // registers: with ctx beside them it also makes -delta and -lse (in log2 units) of its rows and leaves them, [heads][T] each, for the dK / dV kernel.
 // ctx is rounded to bf16, and so is off by 2^-9 of itself, rms, against dP of which it is the mean: nothing beside the rounding of dS where a row sees
-// many keys, but up to twice its effect where it sees a few.  Workgroups with a row of up to 64 keys take delta = sum p dp from a pass of their own over
-// their few tiles instead of from ctx (16 sequences of 1 to 2048: dq off by 2.4e-3 in norm, 2.6e-3 with ctx; short ones alone 2.3e-3 and 4e-3).
+// many keys, but up to twice its effect where it sees a few.  Workgroups with a row that reaches up to 64 keys (masked ones counted) take delta = sum p dp
+// from a pass of their own over their few tiles instead of from ctx (16 sequences of 1 to 2048: dq off by 2.4e-3 in norm, 2.6e-3 with ctx; short ones
+// alone 2.3e-3 and 4e-3).  What the pass costs, forward and backward, 12 heads of 64: 3 sequences of 2047 to 4099 with windows of 16 + 16 82 us against
+// 74, 32 + 32 77 against 74; 256 causal sequences of 1 to 64 69 against 65; the 16 of 1 to 2048 and whole long ones nothing.
 // 4 x 4096 causal, 32 / 8 heads of 128: 765 - 830 us, 3 products of 275 GFLOP, 1.0 PFLOP/s: power again.  64 x 128, 12 heads of 64: 20 us, 76 MB at 3.8 TB/s.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void attn_gqa_dq_kernel(const Args a, const uint16_t* __restrict__ ctx, const uint16_t* __restrict__ dctx,

